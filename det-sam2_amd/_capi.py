@@ -28,6 +28,22 @@ class Ds2Config(C.Structure):
     ]
 
 
+class Ds2Strided(C.Structure):
+    _fields_ = [("p", c_vp), ("s0", C.c_int64), ("s1", C.c_int64), ("s2", C.c_int64)]
+
+
+class Ds2CacheAttentionArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("B", "T", "Hq", "Hkv", "D", "capacity", "prefix_len", "type", "format")] + \
+               [("scale", C.c_float), ("cap", C.c_float)] + \
+               [(n, Ds2Strided) for n in ("q", "k", "v", "k_scales", "v_scales", "prefix_k", "prefix_v", "prefix_k_scales", "prefix_v_scales")] + \
+               [("lens", c_vp), ("slopes", c_vp), ("out", c_vp)]
+
+
+class Ds2AttentionMaskedArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("B", "Lq", "Lk", "Hq", "Hkv", "D", "type", "causal")] + [("scale", C.c_float), ("cap", C.c_float)] + \
+               [(n, Ds2Strided) for n in ("q", "k", "v")] + [(n, c_vp) for n in ("slopes", "lens", "q_start", "prefix", "q_doc", "k_doc", "out")]
+
+
 # name -> (restype, argtypes); must list every symbol include/detsam2_hip.h declares
 SIGNATURES = {
     "ds2_last_error": (C.c_char_p, []),
@@ -77,12 +93,20 @@ SIGNATURES = {
     "ds2_op_layernorm": (C.c_int, [c_vp, c_vp, c_vp, c_vp, i32, i32, C.c_float, i32, c_vp]),
     "ds2_op_attention": (C.c_int, [c_vp, c_vp, c_vp, c_vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float,
                                    i32, i32, i32, i32, i32, i32, i32, c_vp, c_vp, c_vp]),
+    "ds2_op_cache_write": (C.c_int, [i32, C.POINTER(Ds2Strided), C.POINTER(Ds2Strided), C.POINTER(Ds2Strided), i32, i32, i32, i32, i32,
+                                     c_vp, c_vp, i32, i32, c_vp]),
+    "ds2_op_cache_read": (C.c_int, [C.POINTER(Ds2Strided), C.POINTER(Ds2Strided), C.POINTER(Ds2Strided), i32, i32, i32, i32, c_vp, i32,
+                                    i32, c_vp]),
+    "ds2_op_cache_attention_work_bytes": (C.c_int64, [C.POINTER(Ds2CacheAttentionArgs)]),
+    "ds2_op_cache_attention": (C.c_int, [C.POINTER(Ds2CacheAttentionArgs), c_vp, C.c_int64, c_vp]),
+    "ds2_op_attention_masked_work_bytes": (C.c_int64, [C.POINTER(Ds2AttentionMaskedArgs)]),
+    "ds2_op_attention_masked": (C.c_int, [C.POINTER(Ds2AttentionMaskedArgs), c_vp, C.c_int64, c_vp]),
 }
 
 # the PyTorch custom ops csrc/torch_ops.cpp registers (torch.ops.det_sam2.<name>)
 TORCH_OPS = ("ingest_frames", "image_encoder", "bank_assemble", "memory_attention", "sam_heads", "prompt_encoder", "mask_decoder", "memory_encoder",
              "memory_encoder_module", "resize_aa", "mask_prompt_prepare", "obj_ptr_gate", "mask_output",
-             "get_connected_componnets", "fill_holes", "yolo_postprocess")
+             "get_connected_componnets", "fill_holes", "yolo_postprocess", "cache_write", "cache_read", "cache_attention", "attention_masked")
 
 _lib = None
 _ops = None

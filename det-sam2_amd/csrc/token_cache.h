@@ -1,0 +1,43 @@
+// Formats of the token cache (token_cache.hip, cache_attention.h) and the device helpers that its kernels share.
+//
+// A quantised row of D values (D a multiple of 32) is D e4m3 bytes or D / 2 bytes of e2m1 pairs (even element in the low half)
+// plus one scale byte s for every 32 values: value = code * 2^(s - 127).  s is the smallest power of two (at least 2^-126) for
+// which no value of the group exceeds the code's largest one, so nothing saturates and x * 2^(127 - s) is exact: the ONE rounding of
+// a value is the conversion to its code (nearest, ties to even).  s = 255: the group held an infinity or a NaN, all of it reads NaN.
+#pragma once
+#include "common.h"
+#include "../../include/detsam2_hip.h"
+
+#define DS2_CACHE_GROUP 32
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+#ifdef __HIPCC__
+// two fp32 values -> two 16-bit values in a word (round to nearest even)
+template <bool F16>
+__device__ __forceinline__ unsigned ds2_pack16(float a, float b) {
+  if constexpr (F16) return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
+  else return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2_t{a, b}), bf16x2_t));
+}
+template <bool F16>
+__device__ __forceinline__ float ds2_low16(unsigned w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(f16x2_t, w)[0];
+  else return __builtin_bit_cast(float, w << 16);
+}
+template <bool F16>
+__device__ __forceinline__ float ds2_high16(unsigned w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(f16x2_t, w)[1];
+  else return __builtin_bit_cast(float, w & 0xffff0000u);
+}
+
+// scale byte -> the power of two it stands for; 255 -> NaN.  (0 stands for 2^-127, a subnormal: the writer never leaves it, a cache
+// from elsewhere may.)
+__device__ __forceinline__ float ds2_cache_scale(unsigned s) {
+  const unsigned bits = s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23;
+  return __builtin_bit_cast(float, bits);
+}
+#endif

@@ -13,6 +13,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>      // CUDA"): guard / current stream come from the masquerading forms
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <tuple>
 #include <vector>
@@ -376,6 +377,200 @@ std::tuple<Tensor, Tensor> yolo_postprocess(const Tensor& pred, double conf_thre
   return {dets, counts};
 }
 
+// ---- token cache (include/detsam2_hip.h): quantised write / read, attention over it, masked attention of prompts
+int32_t type_of(const Tensor& t, const char* name, bool f32) {
+  const auto st = t.scalar_type();
+  TORCH_CHECK(st == at::kBFloat16 || st == at::kHalf || (f32 && st == at::kFloat), "det_sam2: ", name, " must be bfloat16, float16",
+              f32 ? " or float32" : "", ", got ", toString(st));
+  return st == at::kBFloat16 ? DS2_TYPE_BF16 : st == at::kHalf ? DS2_TYPE_F16 : DS2_TYPE_F32;
+}
+int32_t format_of(c10::string_view f, bool plain) {
+  if (f == "mxfp8") return DS2_CACHE_MXFP8;
+  if (f == "mxfp4") return DS2_CACHE_MXFP4;
+  TORCH_CHECK(plain && f == "plain", "det_sam2: unknown cache format \"", std::string(f.data(), f.size()), "\" (", plain ? "\"plain\", " : "", "\"mxfp8\", \"mxfp4\")");
+  return DS2_CACHE_PLAIN;
+}
+// leading axes as strides (an axis of size 1: 0, whatever the tensor says), last axis contiguous; `lead` of the three axes, from the back
+ds2_strided strided(const Tensor& t, const char* name, const at::Device& dev, int64_t dims = 4) {
+  TORCH_CHECK(t.is_cuda() && t.device() == dev, "det_sam2: ", name, " must be on ", dev);
+  TORCH_CHECK(t.dim() == dims, "det_sam2: ", name, " must have ", dims, " dimensions, got ", t.dim());
+  TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, "det_sam2: the last dimension of ", name, " must be contiguous");
+  int64_t s[3] = {0, 0, 0};
+  for (int64_t i = 0; i + 1 < dims; ++i) s[3 - (dims - 1) + i] = t.size(i) == 1 ? 0 : t.stride(i);
+  return ds2_strided{t.numel() ? t.data_ptr() : nullptr, s[0], s[1], s[2]};
+}
+int32_t int_size(int64_t n, const char* what) {
+  TORCH_CHECK(n <= INT32_MAX, "det_sam2: ", what, " is too large");
+  return (int32_t)n;
+}
+const int32_t* ints(const c10::optional<Tensor>& t, at::IntArrayRef shape, const char* name, const at::Device& dev) {
+  if (!t.has_value()) return nullptr;
+  want(*t, at::kInt, name);
+  TORCH_CHECK(t->device() == dev, "det_sam2: ", name, " must be on ", dev);
+  TORCH_CHECK(t->sizes() == shape, "det_sam2: ", name, " must be int32 ", shape, ", got ", t->sizes());
+  return t->data_ptr<int32_t>();
+}
+void no_overlap(const Tensor& t, const char* name) {
+  // every element of a written tensor has a place of its own: a broadcast axis, or strides that cross, would not
+  int64_t need = 1;
+  std::vector<std::pair<int64_t, int64_t>> ax;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) ax.emplace_back(t.stride(i), t.size(i));
+  std::sort(ax.begin(), ax.end());
+  for (const auto& x : ax) {
+    TORCH_CHECK(x.first >= need, "det_sam2: elements of ", name, " overlap in memory");
+    need = x.first * (x.second - 1) + need;
+  }
+}
+int64_t code_bytes(int32_t format, int64_t D) { return format == DS2_CACHE_MXFP4 ? D / 2 : D; }
+void want_codes(const Tensor& c, const Tensor& s, at::IntArrayRef lead, int64_t D, int32_t format, const char* name) {
+  TORCH_CHECK(c.scalar_type() == at::kByte && s.scalar_type() == at::kByte, "det_sam2: codes and scales of ", name, " must be uint8");
+  std::vector<int64_t> cs(lead.begin(), lead.end()), ss(lead.begin(), lead.end());
+  cs.push_back(code_bytes(format, D));
+  ss.push_back(D / 32);
+  TORCH_CHECK(c.sizes() == at::IntArrayRef(cs), "det_sam2: codes of ", name, " must be ", at::IntArrayRef(cs), ", got ", c.sizes());
+  TORCH_CHECK(s.sizes() == at::IntArrayRef(ss), "det_sam2: scales of ", name, " must be ", at::IntArrayRef(ss), ", got ", s.sizes());
+}
+
+// new rows k (and v) [B,T,H,D] -> codes uint8 [B,H,C,D or D/2], scales uint8 [B,H,C,D/32], in place, at rows pos[b] + t
+void cache_write(const Tensor& k, const c10::optional<Tensor>& v, const Tensor& pos, const c10::optional<Tensor>& count, Tensor k_codes,
+                 Tensor k_scales, c10::optional<Tensor> v_codes, c10::optional<Tensor> v_scales, c10::string_view format) {
+  const int32_t f = format_of(format, false), type = type_of(k, "k", true), n = v.has_value() ? 2 : 1;
+  TORCH_CHECK(v_codes.has_value() == v.has_value() && v_scales.has_value() == v.has_value(), "det_sam2::cache_write: v, v_codes and v_scales go together");
+  TORCH_CHECK(k.dim() == 4 && k_codes.dim() == 4, "det_sam2::cache_write: k [B,T,H,D] and k_codes [B,H,C,D or D/2] expected");
+  const auto dev = k.device();
+  const int64_t B = k.size(0), T = k.size(1), H = k.size(2), D = k.size(3), C = k_codes.size(2);
+  const Tensor* x[2] = {&k, n > 1 ? &*v : nullptr};
+  const Tensor* c[2] = {&k_codes, n > 1 ? &*v_codes : nullptr};
+  const Tensor* s[2] = {&k_scales, n > 1 ? &*v_scales : nullptr};
+  ds2_strided xs[2], cs[2], ss[2];
+  for (int i = 0; i < n; ++i) {
+    const char* name = i ? "v" : "k";
+    TORCH_CHECK(x[i]->sizes() == k.sizes() && x[i]->scalar_type() == k.scalar_type(), "det_sam2::cache_write: k and v must be alike");
+    want_codes(*c[i], *s[i], {B, H, C}, D, f, name);
+    xs[i] = strided(*x[i], name, dev);
+    cs[i] = strided(*c[i], "codes", dev);
+    ss[i] = strided(*s[i], "scales", dev);
+    no_overlap(*c[i], "codes");
+    no_overlap(*s[i], "scales");
+  }
+  const int32_t* p = ints(pos, {B}, "pos", dev);
+  const int32_t* ct = ints(count, {B}, "count", dev);
+  c10::hip::HIPGuardMasqueradingAsCUDA g(dev);
+  check(ds2_op_cache_write(n, xs, cs, ss, int_size(B, "B"), int_size(T, "T"), int_size(H, "H"), int_size(D, "D"), int_size(C, "C"), p, ct, type, f, stream_of(k)),
+        "cache_write");
+}
+
+// codes / scales [B,H,C,...] -> values [B,H,C,D]; rows from lens[b] on are zero
+Tensor cache_read(const Tensor& codes, const Tensor& scales, const c10::optional<Tensor>& lens, c10::string_view format, at::ScalarType dtype) {
+  const int32_t f = format_of(format, false);
+  TORCH_CHECK(codes.is_cuda() && codes.dim() == 4 && scales.dim() == 4, "det_sam2::cache_read: codes / scales [B,H,C,...] on the GPU expected");
+  const int64_t B = codes.size(0), H = codes.size(1), C = codes.size(2), D = codes.size(3) * (f == DS2_CACHE_MXFP4 ? 2 : 1);
+  want_codes(codes, scales, {B, H, C}, D, f, "the cache");
+  const auto dev = codes.device();
+  const ds2_strided cs = strided(codes, "codes", dev), ss = strided(scales, "scales", dev);
+  const int32_t* ln = ints(lens, {B}, "lens", dev);
+  c10::hip::HIPGuardMasqueradingAsCUDA g(dev);
+  Tensor out = at::empty({B, H, C, D}, codes.options().dtype(dtype));
+  const int32_t type = type_of(out, "dtype", true);
+  const ds2_strided os = strided(out, "out", dev);
+  check(ds2_op_cache_read(&cs, &ss, &os, int_size(B, "B"), int_size(H, "H"), int_size(C, "C"), int_size(D, "D"), ln, type, f, stream_of(codes)), "cache_read");
+  return out;
+}
+
+Tensor scratch(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+
+// q [B,T,Hq,D] over k, v [B,Hkv,C,...] and the shared prefix [Hkv,P,...] -> [B,T,Hq,D]
+Tensor cache_attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& k_scales,
+                       const c10::optional<Tensor>& v_scales, const Tensor& lens, const c10::optional<Tensor>& prefix_k,
+                       const c10::optional<Tensor>& prefix_v, const c10::optional<Tensor>& prefix_k_scales,
+                       const c10::optional<Tensor>& prefix_v_scales, c10::string_view format, double scale, double cap,
+                       const c10::optional<Tensor>& slopes) {
+  ds2_cache_attention_args a{};
+  a.format = format_of(format, true);
+  a.type = type_of(q, "q", false);
+  const bool mx = a.format != DS2_CACHE_PLAIN;
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "det_sam2::cache_attention: q [B,T,Hq,D], k / v [B,Hkv,C,...] expected");
+  TORCH_CHECK(k_scales.has_value() == mx && v_scales.has_value() == mx, "det_sam2::cache_attention: scales go with the quantised formats");
+  TORCH_CHECK(prefix_k.has_value() == prefix_v.has_value(), "det_sam2::cache_attention: prefix_k and prefix_v go together");
+  TORCH_CHECK(prefix_k_scales.has_value() == (mx && prefix_k.has_value()) && prefix_v_scales.has_value() == (mx && prefix_k.has_value()),
+              "det_sam2::cache_attention: prefix scales go with a quantised prefix");
+  const auto dev = q.device();
+  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(1), C = k.size(2);
+  TORCH_CHECK(!prefix_k.has_value() || prefix_k->dim() == 3, "det_sam2::cache_attention: prefix_k must be [Hkv,P,...]");
+  const int64_t P = prefix_k.has_value() ? prefix_k->size(1) : 0;
+  auto rows = [&](const Tensor& t, const c10::optional<Tensor>& s, at::IntArrayRef lead, const char* name) {
+    if (mx) want_codes(t, *s, lead, D, a.format, name);
+    else {
+      TORCH_CHECK(t.scalar_type() == q.scalar_type(), "det_sam2::cache_attention: ", name, " must be of q's type");
+      std::vector<int64_t> want(lead.begin(), lead.end());
+      want.push_back(D);
+      TORCH_CHECK(t.sizes() == at::IntArrayRef(want), "det_sam2::cache_attention: ", name, " must be ", at::IntArrayRef(want), ", got ", t.sizes());
+    }
+  };
+  rows(k, k_scales, {B, Hkv, C}, "k");
+  rows(v, v_scales, {B, Hkv, C}, "v");
+  a.q = strided(q, "q", dev), a.k = strided(k, "k", dev), a.v = strided(v, "v", dev);
+  if (mx) a.k_scales = strided(*k_scales, "k_scales", dev), a.v_scales = strided(*v_scales, "v_scales", dev);
+  if (P) {
+    rows(*prefix_k, prefix_k_scales, {Hkv, P}, "prefix_k");
+    rows(*prefix_v, prefix_v_scales, {Hkv, P}, "prefix_v");
+    a.prefix_k = strided(*prefix_k, "prefix_k", dev, 3), a.prefix_v = strided(*prefix_v, "prefix_v", dev, 3);
+    if (mx) a.prefix_k_scales = strided(*prefix_k_scales, "prefix_k_scales", dev, 3), a.prefix_v_scales = strided(*prefix_v_scales, "prefix_v_scales", dev, 3);
+  }
+  a.lens = ints(lens, {B}, "lens", dev);
+  if (slopes.has_value()) {
+    want(*slopes, at::kFloat, "slopes");
+    TORCH_CHECK(slopes->device() == dev && slopes->dim() == 1 && slopes->size(0) == Hq, "det_sam2::cache_attention: slopes must be float32 [Hq] on q's device");
+    a.slopes = slopes->data_ptr<float>();
+  }
+  a.B = int_size(B, "B"), a.T = int_size(T, "T"), a.Hq = int_size(Hq, "Hq"), a.Hkv = int_size(Hkv, "Hkv"), a.D = int_size(D, "D");
+  a.capacity = int_size(C, "C"), a.prefix_len = int_size(P, "P");
+  a.scale = (float)scale, a.cap = (float)cap;
+  c10::hip::HIPGuardMasqueradingAsCUDA g(dev);
+  Tensor out = at::empty({B, T, Hq, D}, q.options());
+  if (!out.numel()) return out;
+  a.out = out.data_ptr();
+  const int64_t bytes = ds2_op_cache_attention_work_bytes(&a);
+  const Tensor work = scratch(bytes, q);
+  check(ds2_op_cache_attention(&a, bytes ? work.data_ptr() : nullptr, bytes, stream_of(q)), "cache_attention");
+  return out;
+}
+
+// q [B,Lq,Hq,D], k / v [B,Lk,Hkv,D] -> [B,Lq,Hq,D]
+Tensor attention_masked(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, double cap,
+                        const c10::optional<Tensor>& slopes, const c10::optional<Tensor>& lens, const c10::optional<Tensor>& q_start,
+                        const c10::optional<Tensor>& prefix, const c10::optional<Tensor>& q_doc, const c10::optional<Tensor>& k_doc) {
+  ds2_attention_masked_args a{};
+  a.type = type_of(q, "q", false);
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(), "det_sam2::attention_masked: q [B,Lq,Hq,D], k / v [B,Lk,Hkv,D] expected");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "det_sam2::attention_masked: q, k and v must be of one type");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(3) == q.size(3), "det_sam2::attention_masked: k ", k.sizes(), " does not go with q ", q.sizes());
+  TORCH_CHECK(q_doc.has_value() == k_doc.has_value(), "det_sam2::attention_masked: q_doc and k_doc go together");
+  TORCH_CHECK(causal || !prefix.has_value(), "det_sam2::attention_masked: a prefix goes with the causal mask");
+  const auto dev = q.device();
+  const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3), Lk = k.size(1);
+  a.q = strided(q, "q", dev), a.k = strided(k, "k", dev), a.v = strided(v, "v", dev);
+  if (slopes.has_value()) {
+    want(*slopes, at::kFloat, "slopes");
+    TORCH_CHECK(slopes->device() == dev && slopes->dim() == 1 && slopes->size(0) == Hq, "det_sam2::attention_masked: slopes must be float32 [Hq] on q's device");
+    a.slopes = slopes->data_ptr<float>();
+  }
+  a.lens = ints(lens, {B}, "lens", dev), a.q_start = ints(q_start, {B}, "q_start", dev), a.prefix = ints(prefix, {B}, "prefix", dev);
+  a.q_doc = ints(q_doc, {B, Lq}, "q_doc", dev), a.k_doc = ints(k_doc, {B, Lk}, "k_doc", dev);
+  a.B = int_size(B, "B"), a.Lq = int_size(Lq, "Lq"), a.Lk = int_size(Lk, "Lk"), a.Hq = int_size(Hq, "Hq"), a.Hkv = int_size(k.size(2), "Hkv");
+  a.D = int_size(D, "D"), a.causal = causal ? 1 : 0;
+  a.scale = (float)scale, a.cap = (float)cap;
+  c10::hip::HIPGuardMasqueradingAsCUDA g(dev);
+  Tensor out = at::empty({B, Lq, Hq, D}, q.options());
+  if (!out.numel()) return out;
+  a.out = out.data_ptr();
+  const int64_t bytes = ds2_op_attention_masked_work_bytes(&a);
+  const Tensor work = scratch(bytes, q);
+  check(ds2_op_attention_masked(&a, bytes ? work.data_ptr() : nullptr, bytes, stream_of(q)), "attention_masked");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(det_sam2, m) {
@@ -397,6 +592,13 @@ TORCH_LIBRARY(det_sam2, m) {
   m.def("get_connected_componnets(Tensor inputs) -> Tensor[]");
   m.def("fill_holes(Tensor logits, int max_area) -> Tensor");
   m.def("yolo_postprocess(Tensor pred, float conf_thres, float iou_thres, int max_det, Tensor? scale5) -> (Tensor, Tensor)");
+  m.def("cache_write(Tensor k, Tensor? v, Tensor pos, Tensor? count, Tensor(a!) k_codes, Tensor(b!) k_scales, Tensor(c!)? v_codes, "
+        "Tensor(d!)? v_scales, str format) -> ()");
+  m.def("cache_read(Tensor codes, Tensor scales, Tensor? lens, str format, ScalarType dtype) -> Tensor");
+  m.def("cache_attention(Tensor q, Tensor k, Tensor v, Tensor? k_scales, Tensor? v_scales, Tensor lens, Tensor? prefix_k, Tensor? prefix_v, "
+        "Tensor? prefix_k_scales, Tensor? prefix_v_scales, str format, float scale, float cap, Tensor? slopes) -> Tensor");
+  m.def("attention_masked(Tensor q, Tensor k, Tensor v, float scale, bool causal, float cap, Tensor? slopes, Tensor? lens, Tensor? q_start, "
+        "Tensor? prefix, Tensor? q_doc, Tensor? k_doc) -> Tensor");
 }
 
 // GPU tensors on PyTorch-ROCm dispatch under the CUDA key (HIP masquerades as CUDA); a CPU tensor finds no kernel and the
@@ -419,4 +621,8 @@ TORCH_LIBRARY_IMPL(det_sam2, CUDA, m) {
   m.impl("get_connected_componnets", &get_connected_componnets);
   m.impl("fill_holes", &fill_holes);
   m.impl("yolo_postprocess", &yolo_postprocess);
+  m.impl("cache_write", &cache_write);
+  m.impl("cache_read", &cache_read);
+  m.impl("cache_attention", &cache_attention);
+  m.impl("attention_masked", &attention_masked);
 }

@@ -306,6 +306,74 @@ int ds2_op_attention(const float* q, const float* k, const float* v, float* o, i
                      float scale, int32_t win_q, int32_t win_k, int32_t Hq, int32_t Wq, int32_t Hk, int32_t Wk,
                      int32_t nwx, const float* k_pad, const float* v_pad, void* stream);
 
+/* ---- token cache: keys and values of a sequence kept in 16, 8 or 4 bits, and the attention that reads them.
+ * A tensor with three leading axes of free strides and a contiguous last one.  Strides count ELEMENTS (codes: bytes); an axis of
+ * size 1 may have any stride that keeps the stated alignment. */
+typedef struct ds2_strided {
+  void* p;
+  int64_t s0, s1, s2;
+} ds2_strided;
+/* element types */
+#define DS2_TYPE_BF16 0
+#define DS2_TYPE_F16 1
+#define DS2_TYPE_F32 2
+/* cache formats: PLAIN = the 16-bit values themselves; MXFP8 = e4m3 codes, one byte a value; MXFP4 = e2m1 codes, the even element
+ * in a byte's low half.  MX rows carry one scale byte s for every 32 values along the head dimension: value = code * 2^(s - 127), s
+ * the smallest (at least 1) for which no value of the group exceeds the largest code (448 resp. 6); codes are rounded to nearest, ties
+ * to even.  A group that holds an infinity or a NaN gets s = 255 and codes 0, and reads back as NaN. */
+#define DS2_CACHE_PLAIN 0
+#define DS2_CACHE_MXFP8 1
+#define DS2_CACHE_MXFP4 2
+
+/* Quantises the new rows of n (1 or 2: keys, values) tensors and writes them behind the tokens that are there:
+ * x[i] [B,T,H,D] (axes b,t,h; type bf16 / fp16 / fp32) -> codes[i] uint8 [B,H,capacity, D or D/2], scales[i] uint8
+ * [B,H,capacity,D/32] (axes b,h,token), token t of sequence b at row pos[b] + t.  pos int32 [B]; count int32 [B] or NULL: only the first
+ * count[b] tokens of a sequence are written.  A token whose row is not in [0, capacity) is not written; no other row is
+ * touched.  D a multiple of 32 up to 4096; rows of x and of codes 16-byte aligned.  x, codes, scales: HOST arrays of n. */
+int ds2_op_cache_write(int32_t n, const ds2_strided* x, const ds2_strided* codes, const ds2_strided* scales, int32_t B, int32_t T,
+                       int32_t H, int32_t D, int32_t capacity, const int32_t* pos, const int32_t* count, int32_t type,
+                       int32_t format, void* stream);
+/* Reads a quantised cache back: out [B,H,C,D] (axes b,h,token) in `type`; rows from lens[b] on (lens int32 [B] or NULL) are zero. */
+int ds2_op_cache_read(const ds2_strided* codes, const ds2_strided* scales, const ds2_strided* out, int32_t B, int32_t H, int32_t C,
+                      int32_t D, const int32_t* lens, int32_t type, int32_t format, void* stream);
+
+/* Attention of the last T tokens of every sequence over its cached tokens and over a prefix that all sequences share:
+ *   o = sum_j softmax_j(s_j) v_j,  s_j = scale q.k_j, then cap tanh(s_j / cap) where cap > 0, then - slopes[h] (distance of the tokens)
+ * q [B,T,Hq,D] (axes b,t,h), bf16 or fp16; k, v [B,Hkv,capacity,D] (axes b,h,token) in `format` (PLAIN: of q's type; MX: codes with
+ * k_scales / v_scales); query head h reads key head h / (Hq / Hkv).  lens int32 [B]: tokens of a sequence in the cache, the T new ones
+ * among them; new token t sees the prefix and its own tokens up to lens[b] - T + t; where that is negative it sees nothing.
+ * prefix_* [Hkv,prefix_len,D] (axes -,h,token; s0 is not used), or prefix_len = 0.  slopes fp32 [Hq] or NULL.  Rows that see nothing are
+ * zero.  out [B,T,Hq,D] contiguous, q's type.  D = 32, 64, 96, 128 or 256; all rows 16-byte aligned (scales: any).
+ * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), which goes by the sizes alone. */
+typedef struct ds2_cache_attention_args {
+  int32_t B, T, Hq, Hkv, D, capacity, prefix_len, type, format;
+  float scale, cap;
+  ds2_strided q, k, v, k_scales, v_scales, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales;
+  const int32_t* lens;
+  const float* slopes;
+  void* out;
+} ds2_cache_attention_args;
+int64_t ds2_op_cache_attention_work_bytes(const ds2_cache_attention_args* args);
+int ds2_op_cache_attention(const ds2_cache_attention_args* args, void* work, int64_t work_bytes, void* stream);
+
+/* Masked attention of whole prompts: q [B,Lq,Hq,D], k, v [B,Lk,Hkv,D] (axes b,token,h), bf16 or fp16, out [B,Lq,Hq,D] contiguous.
+ * Scores as above; the distance of query i and key j is |q_start[b] + i - j| (q_start int32 [B], NULL = 0).  Query i sees key j if
+ *   j < lens[b]                                   (lens int32 [B] or NULL), and
+ *   j <= q_start[b] + i or j < prefix[b]          where causal (prefix int32 [B] or NULL), and
+ *   q_doc[b,i] == k_doc[b,j] and k_doc[b,j] >= 0  where documents are given (int32 [B,Lq] / [B,Lk] contiguous, in any order).
+ * Rows that see nothing are zero.  D a multiple of 8 up to 256; all rows 16-byte aligned.
+ * work: device scratch of ds2_op_attention_masked_work_bytes(args) bytes (0: none needed), which goes by the sizes alone. */
+typedef struct ds2_attention_masked_args {
+  int32_t B, Lq, Lk, Hq, Hkv, D, type, causal;
+  float scale, cap;
+  ds2_strided q, k, v;
+  const float* slopes;
+  const int32_t *lens, *q_start, *prefix, *q_doc, *k_doc;
+  void* out;
+} ds2_attention_masked_args;
+int64_t ds2_op_attention_masked_work_bytes(const ds2_attention_masked_args* args);
+int ds2_op_attention_masked(const ds2_attention_masked_args* args, void* work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
