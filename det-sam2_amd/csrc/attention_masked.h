@@ -1,0 +1,485 @@
+// Masked attention of whole prompts, 16-bit operands, fp32 statistics (kernel templates; instantiated per type in
+// attention_masked_{bf16,f16}.hip):
+//
+//   o_r = sum_j w_rj v_j / sum_j w_rj,  w_rj = exp(s_rj) where row r sees key j, else 0
+//   s = scale q.k, then cap tanh(s / cap), then - slope_h |pos_r - j|
+//
+// One pass with a running maximum and sum.  The rows of a key head are its G Lq (query head, position) pairs, position-major, so that
+// the G heads of a group share every key tile and a tile of rows spans few positions (few edge tiles under the causal mask).
+//
+//  * A wave holds 32 rows: S^T = K Q^T with v_mfma_f32_32x32x16 (A = K from LDS, B = Q in registers) leaves a row's scores in one lane
+//    pair, so maximum and sum cost one exchange.  P^T is the B operand of O^T = V^T P^T straight from the score registers: contraction
+//    slots are free to be permuted, slot j of lane half h is key 8 (j / 4) + 4 h + j % 4 of a block of 16; the A operand
+//    follows with two transposing LDS reads (ds_read_b64_tr_b16: 4 keys of one column a lane).
+//  * Steps of 32 keys, software pipelined: the score products of step i + 1 are issued among the exponentials of step i, the value
+//    products of step i among the scaling (tanh, distance) of step i + 1, so that matrix and vector pipe both have work from one wave.
+//  * Key tiles (64 keys; 32 at head dims over 128) go through registers into one of THREE LDS buffers: loads fly for two tiles, one
+//    barrier a tile.  Rows behind the last key come as zeros from the buffer descriptor's bounds.  K rows are padded by 16 bytes (16 rows
+//    of a ds_read_b128 quarter cover all 64 banks), V rows to 64 bytes modulo 256 (the four rows of a transposing read do).
+//  * causal, prefix and length masks are one number a row: the keys it sees are those below `limit`.  Tiles beyond every row's limit are
+//    not visited, steps below every row's limit are not masked.  Documents: a small kernel notes the smallest and largest document of
+//    each key tile; a wave-wide vote over 64 tiles at a time finds the tiles that can hold a visible pair.
+//  * The running maximum is raised only by more than 2^8: the weights stay below 2^8 and the rescaling of O is rare.
+//  * Weights are rounded to the operands' 16-bit type before the value product (one rounding of half a step, like the output's own);
+//    their sum takes the unrounded ones.
+#pragma once
+#include "token_cache.h"
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
+
+// Over 128 output elements a row, two waves take half of them each and both compute the scores: 128 accumulators and 64 query
+// registers a wave leave no room for the pipeline.
+constexpr int masked_value_split(int D) { return D > 128 ? 2 : 1; }
+constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }     // keys of a tile
+constexpr float LOG2E = 1.44269504088896340736f;
+enum { MASKED_PLAIN = 0, MASKED_CAP = 1, MASKED_SLOPES = 2 };      // how scores become exponents (SLOPES: cap too, if it is set)
+
+}  // namespace
+
+struct MaskedArgs {
+  const char *q, *k, *v;
+  char* out;
+  int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;    // bytes
+  const float* slopes;
+  const int32_t *lens, *q_start, *prefix, *q_doc, *k_doc;
+  const int2* tile_docs;                    // [B][tiles]: smallest (-1: a key of none among them) and largest document of a tile
+  int B, Lq, Lk, Hq, Hkv, G, D, causal;
+  float scale, cap;
+  int row_tiles, heads, parts, tiles, tiles_a_part;
+  float* part_o;                            // null: one part
+  f32x2_t* part_ml;
+};
+
+int launch_masked_bf16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
+int launch_masked_f16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
+
+namespace {
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+// 16-bit pair: which halves are infinities or NaNs, as a mask over the word
+template <bool F16>
+__device__ __forceinline__ unsigned not_finite(unsigned w) {
+  constexpr unsigned EXP = F16 ? 0x7c00u : 0x7f80u;
+  return ((w & EXP) == EXP ? 0xffffu : 0u) | (((w >> 16) & EXP) == EXP ? 0xffff0000u : 0u);
+}
+
+// The register limit keeps accumulators out of the AGPRs.  With them, and a divergent branch in the tile loop, hipcc placed copies into
+// AGPRs in front of the restored lane mask; the loop below has wave-uniform branches only.
+template <bool F16, int DP, int MODE>
+__global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void k_attn_masked(MaskedArgs a) {
+  constexpr int NW = 8;                                          // waves (those without rows of their own stage keys for the others)
+  constexpr int KT = masked_tile(DP), H = KT / 32;               // steps of a tile
+  constexpr int VS = masked_value_split(DP), RW = NW / VS;       // waves that share rows (each takes 1 / VS of the output), waves of other rows
+  constexpr int KS = DP / 16, DB = DP / 32 / VS;                 // contraction steps of a score, a wave's blocks of 32 output elements
+  constexpr int KROW = DP * 2 + 16, VROW = DP == 32 ? 64 : DP == 64 ? 192 : DP == 96 ? 192 : DP == 128 ? 320 : 576;
+  constexpr int CH = DP / 8;                                     // 16-byte pieces of a row
+  constexpr int NT = NW * 64, PER = (KT * CH + NT - 1) / NT;     // pieces a thread stages of a K (and of a V) tile
+  __shared__ __attribute__((aligned(16))) unsigned char lk[3][KT * KROW + 16];     // (+ 16: where threads without a piece write)
+  __shared__ __attribute__((aligned(16))) unsigned char lv[3][KT * VROW + 16];
+  __shared__ int ldoc[3][64];
+  __shared__ int wg_lim[NW][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+
+  // ---- which tile: the heads of a batch are spread over the chiplets (blockIdx % 8), long row tiles first
+  int id = blockIdx.x, part = 0, head, rt;
+  {
+    const int nh = a.heads, total = nh * a.parts;
+    if (nh % 8 == 0) {
+      const int x = id & 7, y = id >> 3, per = total / 8;
+      const int z = y % per;
+      rt = a.row_tiles - 1 - y / per;
+      head = x * (nh / 8) + z / a.parts, part = z % a.parts;
+    } else {
+      rt = a.row_tiles - 1 - id / total;
+      const int z = id % total;
+      head = z / a.parts, part = z % a.parts;
+    }
+  }
+  const int b = head / a.Hkv, kvh = head - b * a.Hkv;
+  const int rows = a.G * a.Lq;
+  const int row0 = rt * RW * 32 + wave % RW * 32;                // the wave's rows of this key head
+  const int d0 = wave / RW * DB * 32;                            // and its first output element
+  const int r = min(row0 + c, rows - 1);                         // rows behind the last repeat it and are not written
+  const int i = r / a.G, hq = kvh * a.G + (r - i * a.G);
+  const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
+  const int64_t pos = (int64_t)(a.q_start ? a.q_start[b] : 0) + i;
+  const float slope = MODE == MASKED_SLOPES && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
+  int limit = len;
+  if (a.causal) {
+    int64_t n = pos + 1;
+    if (a.prefix) n = max(n, (int64_t)a.prefix[b]);
+    limit = (int)max((int64_t)0, min((int64_t)len, n));
+  }
+  const int qdoc = a.q_doc ? a.q_doc[(int64_t)b * a.Lq + i] : 0;
+
+  // ---- smallest and largest limit and document of the wave and of the workgroup
+  int lo = limit, hi = limit, dlo = qdoc, dhi = qdoc;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s));
+    dlo = min(dlo, __shfl_xor(dlo, s)), dhi = max(dhi, __shfl_xor(dhi, s));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+  dlo = __builtin_amdgcn_readfirstlane(dlo), dhi = __builtin_amdgcn_readfirstlane(dhi);
+  if (lane == 0) wg_lim[wave][0] = lo, wg_lim[wave][1] = hi, wg_lim[wave][2] = dlo, wg_lim[wave][3] = dhi;
+  __syncthreads();
+  int ghi = 0, gdlo = INT32_MAX, gdhi = -1;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) ghi = max(ghi, wg_lim[w][1]), gdlo = min(gdlo, wg_lim[w][2]), gdhi = max(gdhi, wg_lim[w][3]);
+  ghi = __builtin_amdgcn_readfirstlane(ghi), gdlo = __builtin_amdgcn_readfirstlane(gdlo), gdhi = __builtin_amdgcn_readfirstlane(gdhi);
+
+  const int t_end = min((ghi + KT - 1) / KT, (part + 1) * a.tiles_a_part);
+  const int t_begin = part * a.tiles_a_part;
+  // next tile at or behind t that may hold a visible pair (the same answer in every wave); t_end: none.  64 tiles are looked at a time,
+  // one a lane, and kept.
+  const int2* td = a.tile_docs ? a.tile_docs + (int64_t)b * a.tiles : nullptr;
+  int window = -64;
+  unsigned long long window_on = 0;
+  int2 mine = {-1, -1};
+  auto next_tile = [&](int t) {
+    if (!td) return min(t, t_end);
+    while (t < t_end) {
+      if (t >= window + 64) {
+        window = t;
+        mine = t + lane < t_end ? td[t + lane] : int2{-1, -1};
+        window_on = __ballot(gdhi >= 0 && mine.x <= gdhi && mine.y >= max(gdlo, 0));
+      }
+      const unsigned long long on = window_on >> (t - window);
+      if (on) return t + __builtin_ctzll(on);
+      t = window + 64;
+    }
+    return t_end;
+  };
+  // the one document of the tile that next_tile has just found; -1: several, or keys of none
+  auto tile_doc = [&](int t) {
+    if (!td || t >= t_end) return -1;
+    const int x = __builtin_amdgcn_readlane(mine.x, t - window), y = __builtin_amdgcn_readlane(mine.y, t - window);
+    return x == y ? x : -1;
+  };
+
+  // ---- queries
+  u32x4 qf[KS];
+  {
+    const char* row = a.q + b * a.q_b + (int64_t)i * a.q_t + hq * a.q_h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * h;
+      qf[s] = d < a.D ? *(const u32x4*)(row + d * 2) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));  // (arrived here: a wait inside the loop would be for the tile loads too)
+  }
+
+  // ---- staging
+  const char *kb = a.k + b * a.k_b + kvh * a.k_h, *vb = a.v + b * a.v_b + kvh * a.v_h;
+  unsigned k_off[PER], v_off[PER];                               // of the thread's pieces in a tile; beyond any bound where there are none
+  int lds_k[PER], lds_v[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int p = u * NT + tid, row = p / CH, piece = p - row * CH;
+    const bool place = PER * NT == KT * CH || row < KT, live = place && piece * 8 < a.D;
+    k_off[u] = live ? (unsigned)(row * (int)a.k_t + piece * 16) : 0x80000000u;
+    v_off[u] = live ? (unsigned)(row * (int)a.v_t + piece * 16) : 0x80000000u;
+    lds_k[u] = place ? row * KROW + piece * 16 : KT * KROW, lds_v[u] = place ? row * VROW + piece * 16 : KT * VROW;
+  }
+  u32x4 sk[PER], sv[PER];
+  int sdoc = -1;
+  auto fetch = [&](int t) {                                      // a tile into registers; behind the last key: zeros
+    const int left = len - t * KT;                               // > 0
+    const int64_t kn = (int64_t)(min(left, KT) - 1) * a.k_t + a.D * 2, vn = (int64_t)(min(left, KT) - 1) * a.v_t + a.D * 2;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (int64_t)t * KT * a.k_t), 0, (int)kn, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (int64_t)t * KT * a.v_t), 0, (int)vn, 0x00020000);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      sk[u] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[u], 0, 0);
+      sv[u] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[u], 0, 0);
+    }
+    if (td) {                                                    // (every wave fetches and writes all of the tile's documents: no divergent branch)
+      const __amdgpu_buffer_rsrc_t dr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k_doc + (int64_t)b * a.Lk + t * KT), 0, min(left, KT) * 4, 0x00020000);
+      sdoc = __builtin_amdgcn_raw_buffer_load_b32(dr, lane * 4, 0, 0);
+      sdoc = lane < left ? sdoc : -1;
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      *(u32x4*)(lk[buf] + lds_k[u]) = sk[u];
+      *(u32x4*)(lv[buf] + lds_v[u]) = sv[u];
+    }
+    if (td) ldoc[buf][lane] = sdoc;
+  };
+
+  // ---- pieces of a step
+  const float sc = a.scale * LOG2E, cap2 = a.cap * LOG2E, in_cap = a.cap > 0.f ? 2.f * LOG2E * a.scale / a.cap : 0.f;
+  const unsigned k_lane = c * KROW + h * 16;
+  const unsigned v_lane = (4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4 & 1) * 16 + 4 * (lane & 3) + d0) * 2;
+  f32x16 o[DB];
+  float m, l;
+  auto clear = [&]() {
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 16; ++y) o[x][y] = 0.f;
+    m = -INFINITY, l = 0.f;
+  };
+  auto scores = [&](f32x16& s, int buf, int half) {
+#pragma unroll
+    for (int y = 0; y < 16; ++y) s[y] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma32<F16>(*(const u32x4*)(lk[buf] + half * 32 * KROW + k_lane + ks * 32), qf[ks], s);
+  };
+  auto exponents = [&](f32x16& s, int key0) {                    // scores -> base-2 exponents (PLAIN: left to the exponential's fma)
+    if constexpr (MODE == MASKED_PLAIN) return;
+    if (MODE == MASKED_CAP || a.cap > 0.f) {
+      // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)): no branch, saturates by itself; off by a few 2^-24 of cap
+#pragma unroll
+      for (int y = 0; y < 16; ++y)
+        s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 16; ++y) s[y] *= sc;
+    }
+    if constexpr (MODE == MASKED_SLOPES) {
+      const float rel = (float)(int)(pos - key0 - 4 * h);
+#pragma unroll
+      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-slope, fabsf(rel - (float)(8 * (y >> 2) + (y & 3))), s[y]);
+    }
+  };
+  auto hide = [&](f32x16& s, int key0, int buf, int half) {
+    const int rel = limit - key0 - 4 * h;
+#pragma unroll
+    for (int y = 0; y < 16; ++y)
+      if (8 * (y >> 2) + (y & 3) >= rel) s[y] = -INFINITY;
+    if (td) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const u32x4 d = *(const u32x4*)&ldoc[buf][32 * half + 8 * y + 4 * h];
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if ((int)d[z] != qdoc || qdoc < 0) s[4 * y + z] = -INFINITY;
+      }
+    }
+  };
+  constexpr bool RAW = MODE == MASKED_PLAIN;                     // exponents still lack the factor sc
+  auto raise = [&](const f32x16& s) {
+    float top = s[0];
+#pragma unroll
+    for (int y = 1; y < 16; ++y) top = fmaxf(top, s[y]);
+    if (RAW) top *= sc;
+    if (__any(top > m + 8.f)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float mn = fmaxf(m, top);
+      const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= al;
+#pragma unroll
+      for (int x = 0; x < DB; ++x)
+#pragma unroll
+        for (int y = 0; y < 16; ++y) o[x][y] *= al;
+      m = mn;
+    }
+  };
+  auto weights = [&](f32x16& s) {
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int y = 0; y < 16; ++y) {
+      s[y] = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[y], sc, -ref) : s[y] - ref);
+      l += s[y];
+    }
+  };
+  auto packed = [&](const f32x16& s, int kk) {                   // weights of 16 keys as an operand
+    u32x4 p;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) p[y] = ds2_pack16<F16>(s[8 * kk + 2 * y], s[8 * kk + 2 * y + 1]);
+    return p;
+  };
+  auto value_operand = [&](int buf, int half, int kk, int x) {
+    const unsigned char* at = lv[buf] + v_lane + (half * 32 + kk * 16) * VROW + x * 64;
+    const u32x2 w0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at));
+    const u32x2 w1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * VROW)));
+    return u32x4{w0[0], w0[1], w1[0], w1[1]};
+  };
+  auto is_edge = [&](int doc, int key0) {                        // some row of the wave may not see all of the step's keys
+    return key0 + 32 > lo || (td && (doc < 0 || dlo != dhi || dlo != doc));
+  };
+
+  if (row0 >= rows) hi = 0;                                      // no rows of its own: stages keys for the others
+  // ---- main loop: tile t0 in use, t1 in LDS, t2 in registers
+  clear();
+  bool edges = false;
+  int t0 = next_tile(t_begin), doc0 = tile_doc(t0);
+  if (t0 < t_end) {
+    int t1 = next_tile(t0 + 1), doc1 = tile_doc(t1), t2 = next_tile(t1 + 1), doc2 = tile_doc(t2), t3 = t_end, doc3 = -1, buf = 0;
+    fetch(t0);
+    stage(0);
+    if (t1 < t_end) {
+      fetch(t1);
+      stage(1);
+    }
+    if (t2 < t_end) fetch(t2);
+    __syncthreads();
+    f32x16 s;
+    scores(s, 0, 0);
+    exponents(s, t0 * KT);
+    while (true) {
+      const int next = buf == 2 ? 0 : buf + 1;
+#pragma unroll
+      for (int half = 0; half < H; ++half) {
+        const int key0 = t0 * KT + half * 32;
+        if (key0 < hi) {                                         // (keys ascend: a wave that is done stays done)
+          // (The edge is decided before any product: no branch between score products and their first use - hipcc left out the wait
+          // states in front of an accumulator read behind such a branch, and the last product's terms were missing.)
+          if (is_edge(doc0, key0)) {
+            edges = true;
+            hide(s, key0, buf, half);
+          }
+          raise(s);
+          f32x16 n;
+          scores(n, half + 1 < H ? buf : next, half + 1 < H ? half + 1 : 0);   // (behind the last tile: not used)
+          weights(s);
+          const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
+#pragma unroll
+          for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
+#pragma unroll
+          for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 1, x), p1, o[x]);
+          exponents(n, half + 1 < H ? key0 + 32 : t1 * KT);
+          s = n;
+        }
+        if (half == 0) {
+          if (t2 < t_end) stage(next == 2 ? 0 : next + 1);       // (that buffer was last read before this tile's barrier)
+          t3 = next_tile(t2 + 1), doc3 = tile_doc(t3);
+          if (t3 < t_end) fetch(t3);
+        }
+      }
+      if (t1 >= t_end) break;
+      __syncthreads();
+      t0 = t1, t1 = t2, t2 = t3, doc0 = doc1, doc1 = doc2, doc2 = doc3, buf = next;
+    }
+  }
+
+  // ---- A hidden key has weight 0, but 0 times an infinity or a NaN is not 0.  Only edge steps can hide a key from some of the rows; if a
+  // result is not finite after one, the tile is computed again, and values that are not finite go to the rows that see them one by
+  // one (rare: speed does not matter).
+  {
+    float z = 0.f;
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 16; ++y) z = __builtin_fmaf(o[x][y], 0.f, z);
+    const bool bad = __any(!(z == 0.f)) && edges;
+    __syncthreads();
+    if (lane == 0) wg_lim[wave][0] = bad;
+    __syncthreads();
+    int again = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) again |= wg_lim[w][0];
+    if (__builtin_amdgcn_readfirstlane(again)) {
+      clear();
+      window = -64, window_on = 0;
+      for (int t = next_tile(t_begin); t < t_end; t = next_tile(t + 1)) {
+        const int doc = tile_doc(t);
+        __syncthreads();
+        fetch(t);
+        stage(0);
+        __syncthreads();
+#pragma unroll 1
+        for (int half = 0; half < H; ++half) {
+          const int key0 = t * KT + half * 32;
+          if (key0 >= hi) break;
+          const bool edge = is_edge(doc, key0);
+          f32x16 s;
+          scores(s, 0, half);
+          exponents(s, key0);
+          if (edge) hide(s, key0, 0, half);
+          raise(s);
+          weights(s);
+          if (edge) {
+#pragma unroll 1
+            for (int key = 0; key < 32; ++key) {
+              const int want = (key & 3) | (key >> 3) << 2;
+              float w = 0.f;
+#pragma unroll
+              for (int y = 0; y < 16; ++y) w = want == y ? s[y] : w;
+              w = __shfl(w, c | (key >> 2 & 1) << 5);
+              if (key0 + key >= limit || (td && (ldoc[0][32 * half + key] != qdoc || qdoc < 0))) continue;
+#pragma unroll
+              for (int x = 0; x < DB; ++x)
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                  const float v = ds2_low16<F16>(*(const uint16_t*)(lv[0] + (half * 32 + key) * VROW + (d0 + x * 32 + 8 * (y >> 2) + 4 * h + (y & 3)) * 2));
+                  if (!__builtin_isfinite(v)) o[x][y] += w * v;
+                }
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk) {
+            const u32x4 p = packed(s, kk);
+#pragma unroll
+            for (int x = 0; x < DB; ++x) {
+              u32x4 v = value_operand(0, half, kk, x);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) v[y] &= edge ? ~not_finite<F16>(v[y]) : 0xffffffffu;
+              o[x] = mfma32<F16>(v, p, o[x]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  if (row0 + c >= rows) return;
+  const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + hq;
+  const bool none = m == -INFINITY && l == 0.f;                  // nothing seen: zeros
+  if (a.part_o) {
+    const int64_t at = (int64_t)part * a.B * a.Lq * a.Hq + row;
+    if (h == 0 && d0 == 0) a.part_ml[at] = f32x2_t{m, l};
+    if (none) return;                                            // the join does not read such a row
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int d = d0 + x * 32 + 8 * y + 4 * h;
+        if (d < a.D) *(f32x4*)(a.part_o + at * a.D + d) = f32x4{o[x][4 * y], o[x][4 * y + 1], o[x][4 * y + 2], o[x][4 * y + 3]};
+      }
+  } else {
+    const float f = none ? 0.f : 1.f / l;
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int d = d0 + x * 32 + 8 * y + 4 * h;
+        if (d < a.D)
+          *(u32x2*)(a.out + (row * a.D + d) * 2) = none ? u32x2{0, 0}
+                                                        : u32x2{ds2_pack16<F16>(o[x][4 * y] * f, o[x][4 * y + 1] * f), ds2_pack16<F16>(o[x][4 * y + 2] * f, o[x][4 * y + 3] * f)};
+      }
+  }
+}
+
+template <bool F16, int DP>
+void launch_masked_mode(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
+  if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP><<<dim3(blocks), 512, 0, st>>>(a);
+  else k_attn_masked<F16, DP, MASKED_SLOPES><<<dim3(blocks), 512, 0, st>>>(a);
+}
+template <bool F16>
+int launch_masked(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
+  if (a.D <= 32) launch_masked_mode<F16, 32>(a, mode, blocks, st);
+  else if (a.D <= 64) launch_masked_mode<F16, 64>(a, mode, blocks, st);
+  else if (a.D <= 96) launch_masked_mode<F16, 96>(a, mode, blocks, st);
+  else if (a.D <= 128) launch_masked_mode<F16, 128>(a, mode, blocks, st);
+  else launch_masked_mode<F16, 256>(a, mode, blocks, st);
+  DS2_CHECK_LAUNCH();
+  return DS2_OK;
+}
+
+}  // namespace

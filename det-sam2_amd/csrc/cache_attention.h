@@ -346,7 +346,7 @@ struct CacheStream {
 };
 
 template <int FORMAT, bool QF16, int E, int RT, bool FULL>
-__global__ __launch_bounds__(256) void k_cache_attn(CacheAttnArgs a) {
+__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void k_cache_attn(CacheAttnArgs a) {
   typedef CacheStream<FORMAT, QF16, E, RT, FULL> Stream;
   constexpr bool HALF = QF16;
   __shared__ float join[3][RT * E * 4 + 2 * RT][64];
