@@ -20,8 +20,7 @@
 //    not visited, steps below every row's limit are not masked.  Documents: a small kernel notes the smallest and largest document of
 //    each key tile; a wave-wide vote over 64 tiles at a time finds the tiles that can hold a visible pair.
 //  * The running maximum is raised only by more than 2^8: the weights stay below 2^8 and the rescaling of O is rare.
-//  * Weights are rounded to the operands' 16-bit type before the value product (one rounding of half a step, like the output's own);
-//    their sum takes the unrounded ones.
+//  * Weights are rounded to the operands' 16-bit type before the value product: one rounding of half a step, like the output's own.
 #pragma once
 #include "token_cache.h"
 
@@ -50,7 +49,7 @@ struct MaskedArgs {
   const int2* tile_docs;                    // [B][tiles]: smallest (-1: a key of none among them) and largest document of a tile
   int B, Lq, Lk, Hq, Hkv, G, D, causal;
   float scale, cap;
-  int row_tiles, heads, parts, tiles, tiles_a_part;
+  int row_tiles, heads, parts, tiles, tiles_a_part, fold;
   float* part_o;                            // null: one part
   f32x2_t* part_ml;
 };
@@ -75,7 +74,7 @@ __device__ __forceinline__ unsigned not_finite(unsigned w) {
 // The register limit keeps accumulators out of the AGPRs.  With them, and a divergent branch in the tile loop, hipcc placed copies into
 // AGPRs in front of the restored lane mask; the loop below has wave-uniform branches only.
 template <bool F16, int DP, int MODE>
-__global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void k_attn_masked(MaskedArgs a) {
+__global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs a) {
   constexpr int NW = 8;                                          // waves (those without rows of their own stage keys for the others)
   constexpr int KT = masked_tile(DP), H = KT / 32;               // steps of a tile
   constexpr int VS = masked_value_split(DP), RW = NW / VS;       // waves that share rows (each takes 1 / VS of the output), waves of other rows
@@ -90,20 +89,23 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
 
-  // ---- which tile: the heads of a batch are spread over the chiplets (blockIdx % 8), long row tiles first
+  // ---- which tile: the heads of a batch are spread over the chiplets (blockIdx % 8); row tiles in descending order, the longest
+  // of a causal mask first.  (fold: all workgroups are resident at once, two a CU; the second half ascends, so that a long and a
+  // short one meet.)
   int id = blockIdx.x, part = 0, head, rt;
   {
     const int nh = a.heads, total = nh * a.parts;
     if (nh % 8 == 0) {
       const int x = id & 7, y = id >> 3, per = total / 8;
       const int z = y % per;
-      rt = a.row_tiles - 1 - y / per;
+      rt = y / per;
       head = x * (nh / 8) + z / a.parts, part = z % a.parts;
     } else {
-      rt = a.row_tiles - 1 - id / total;
+      rt = id / total;
       const int z = id % total;
       head = z / a.parts, part = z % a.parts;
     }
+    rt = a.fold && rt >= (a.row_tiles + 1) / 2 ? rt - (a.row_tiles + 1) / 2 : a.row_tiles - 1 - rt;
   }
   const int b = head / a.Hkv, kvh = head - b * a.Hkv;
   const int rows = a.G * a.Lq;
@@ -112,26 +114,28 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
   const int r = min(row0 + c, rows - 1);                         // rows behind the last repeat it and are not written
   const int i = r / a.G, hq = kvh * a.G + (r - i * a.G);
   const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
-  const int64_t pos = (int64_t)(a.q_start ? a.q_start[b] : 0) + i;
+  const int start = a.q_start ? max(-(1 << 30), min(a.q_start[b], 1 << 30)) : 0;
+  const int pos = start + i;
   const float slope = MODE == MASKED_SLOPES && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
   int limit = len;
   if (a.causal) {
-    int64_t n = pos + 1;
-    if (a.prefix) n = max(n, (int64_t)a.prefix[b]);
-    limit = (int)max((int64_t)0, min((int64_t)len, n));
+    int n = pos + 1;
+    if (a.prefix) n = max(n, a.prefix[b]);
+    limit = max(0, min(len, n));
   }
-  const int qdoc = a.q_doc ? a.q_doc[(int64_t)b * a.Lq + i] : 0;
+  int qdoc = a.q_doc ? a.q_doc[(int64_t)b * a.Lq + i] : 0;
+  qdoc = qdoc < 0 ? -2 : qdoc;                                   // of no document: equal to no key's (a key of none is -1 in LDS)
 
-  // ---- smallest and largest limit and document of the wave and of the workgroup
-  int lo = limit, hi = limit, dlo = qdoc, dhi = qdoc;
+  // ---- smallest and largest limit and document of the wave and of the workgroup (rows of no document do not widen the range)
+  int lo = limit, hi = limit, dlo = qdoc < 0 ? INT32_MAX : qdoc, dhi = qdoc, dmin = qdoc;
 #pragma unroll
   for (int s = 1; s < 32; s <<= 1) {
-    lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s));
+    lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s)), dmin = min(dmin, __shfl_xor(dmin, s));
     dlo = min(dlo, __shfl_xor(dlo, s)), dhi = max(dhi, __shfl_xor(dhi, s));
   }
   lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-  dlo = __builtin_amdgcn_readfirstlane(dlo), dhi = __builtin_amdgcn_readfirstlane(dhi);
-  if (lane == 0) wg_lim[wave][0] = lo, wg_lim[wave][1] = hi, wg_lim[wave][2] = dlo, wg_lim[wave][3] = dhi;
+  dmin = __builtin_amdgcn_readfirstlane(dmin), dhi = __builtin_amdgcn_readfirstlane(dhi);
+  if (lane == 0) wg_lim[wave][1] = hi, wg_lim[wave][2] = dlo, wg_lim[wave][3] = dhi;
   __syncthreads();
   int ghi = 0, gdlo = INT32_MAX, gdhi = -1;
 #pragma unroll
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
       if (t >= window + 64) {
         window = t;
         mine = t + lane < t_end ? td[t + lane] : int2{-1, -1};
-        window_on = __ballot(gdhi >= 0 && mine.x <= gdhi && mine.y >= max(gdlo, 0));
+        window_on = __ballot(gdhi >= 0 && mine.x <= gdhi && mine.y >= gdlo);
       }
       const unsigned long long on = window_on >> (t - window);
       if (on) return t + __builtin_ctzll(on);
@@ -207,7 +211,7 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
     if (td) {                                                    // (every wave fetches and writes all of the tile's documents: no divergent branch)
       const __amdgpu_buffer_rsrc_t dr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k_doc + (int64_t)b * a.Lk + t * KT), 0, min(left, KT) * 4, 0x00020000);
       sdoc = __builtin_amdgcn_raw_buffer_load_b32(dr, lane * 4, 0, 0);
-      sdoc = lane < left ? sdoc : -1;
+      sdoc = lane < left ? max(sdoc, -1) : -1;
     }
   };
   auto stage = [&](int buf) {
@@ -238,44 +242,63 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) s = mfma32<F16>(*(const u32x4*)(lk[buf] + half * 32 * KROW + k_lane + ks * 32), qf[ks], s);
   };
-  auto exponents = [&](f32x16& s, int key0) {                    // scores -> base-2 exponents (PLAIN: left to the exponential's fma)
-    if constexpr (MODE == MASKED_PLAIN) return;
-    if (MODE == MASKED_CAP || a.cap > 0.f) {
-      // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)): no branch, saturates by itself; off by a few 2^-24 of cap
+  // scores -> values whose exponent (base 2) is factor * value + offset: PLAIN the scores themselves; CAP 1 / (1 + exp(2 x / cap)), as
+  // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)) (no branch, saturates by itself; off by a few 2^-24 of cap); SLOPES
+  // exponents up to the bias of the lane's first key, which is returned.
+  constexpr bool DOWN = MODE == MASKED_CAP;                      // the largest exponent has the smallest value
+  const float factor = MODE == MASKED_PLAIN ? sc : -2.f * cap2;
+  const int pos_first = start + min(row0, rows - 1) / a.G, pos_last = start + min(row0 + 31, rows - 1) / a.G;   // of the wave's rows
+  auto exponents = [&](f32x16& s, int key0) {
+    if constexpr (MODE == MASKED_PLAIN) return 0.f;
+    if constexpr (MODE == MASKED_CAP) {
 #pragma unroll
-      for (int y = 0; y < 16; ++y)
-        s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
-    } else {
-#pragma unroll
-      for (int y = 0; y < 16; ++y) s[y] *= sc;
+      for (int y = 0; y < 16; ++y) s[y] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap));
+      return cap2;
     }
-    if constexpr (MODE == MASKED_SLOPES) {
-      const float rel = (float)(int)(pos - key0 - 4 * h);
+    float f = sc;
+    if (a.cap > 0.f) {
 #pragma unroll
-      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-slope, fabsf(rel - (float)(8 * (y >> 2) + (y & 3))), s[y]);
+      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
+      f = 1.f;
     }
+    const float rel = (float)(pos - key0 - 4 * h);          // distance of the lane's first key
+    if (key0 + 31 <= pos_first) {                                // all keys before all rows: the bias is linear in the key
+#pragma unroll
+      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(slope, (float)(8 * (y >> 2) + (y & 3)), s[y] * f);
+      return -slope * rel;
+    }
+    if (key0 >= pos_last) {                                      // all keys behind
+#pragma unroll
+      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(slope, -(float)(8 * (y >> 2) + (y & 3)), s[y] * f);
+      return slope * rel;
+    }
+#pragma unroll
+    for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-slope, fabsf(rel - (float)(8 * (y >> 2) + (y & 3))), s[y] * f);
+    return 0.f;
   };
   auto hide = [&](f32x16& s, int key0, int buf, int half) {
-    const int rel = limit - key0 - 4 * h;
+    constexpr float NEVER = DOWN ? INFINITY : -INFINITY;
+    if (key0 + 32 > lo) {
+      const int rel = limit - key0 - 4 * h;
 #pragma unroll
-    for (int y = 0; y < 16; ++y)
-      if (8 * (y >> 2) + (y & 3) >= rel) s[y] = -INFINITY;
+      for (int y = 0; y < 16; ++y)
+        if (8 * (y >> 2) + (y & 3) >= rel) s[y] = NEVER;
+    }
     if (td) {
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const u32x4 d = *(const u32x4*)&ldoc[buf][32 * half + 8 * y + 4 * h];
 #pragma unroll
         for (int z = 0; z < 4; ++z)
-          if ((int)d[z] != qdoc || qdoc < 0) s[4 * y + z] = -INFINITY;
+          if ((int)d[z] != qdoc) s[4 * y + z] = NEVER;
       }
     }
   };
-  constexpr bool RAW = MODE == MASKED_PLAIN;                     // exponents still lack the factor sc
-  auto raise = [&](const f32x16& s) {
+  auto raise = [&](const f32x16& s, float offset) {
     float top = s[0];
 #pragma unroll
-    for (int y = 1; y < 16; ++y) top = fmaxf(top, s[y]);
-    if (RAW) top *= sc;
+    for (int y = 1; y < 16; ++y) top = DOWN ? fminf(top, s[y]) : fmaxf(top, s[y]);
+    top = MODE == MASKED_SLOPES ? top + offset : __builtin_fmaf(top, factor, offset);
     if (__any(top > m + 8.f)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m, top);
@@ -288,11 +311,11 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
       m = mn;
     }
   };
-  auto weights = [&](f32x16& s) {
-    const float ref = m == -INFINITY ? 0.f : m;
+  auto weights = [&](f32x16& s, float offset) {
+    const float off = offset - (m == -INFINITY ? 0.f : m);
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
-      s[y] = __builtin_amdgcn_exp2f(RAW ? __builtin_fmaf(s[y], sc, -ref) : s[y] - ref);
+      s[y] = __builtin_amdgcn_exp2f(MODE == MASKED_SLOPES ? s[y] + off : __builtin_fmaf(s[y], factor, off));
       l += s[y];
     }
   };
@@ -309,7 +332,7 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
     return u32x4{w0[0], w0[1], w1[0], w1[1]};
   };
   auto is_edge = [&](int doc, int key0) {                        // some row of the wave may not see all of the step's keys
-    return key0 + 32 > lo || (td && (doc < 0 || dlo != dhi || dlo != doc));
+    return key0 + 32 > lo || (td && (doc < 0 || dmin != dhi || dmin != doc));
   };
 
   if (row0 >= rows) hi = 0;                                      // no rows of its own: stages keys for the others
@@ -329,7 +352,7 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
     __syncthreads();
     f32x16 s;
     scores(s, 0, 0);
-    exponents(s, t0 * KT);
+    float offset = exponents(s, t0 * KT);
     while (true) {
       const int next = buf == 2 ? 0 : buf + 1;
 #pragma unroll
@@ -342,16 +365,16 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
             edges = true;
             hide(s, key0, buf, half);
           }
-          raise(s);
+          raise(s, offset);
           f32x16 n;
           scores(n, half + 1 < H ? buf : next, half + 1 < H ? half + 1 : 0);   // (behind the last tile: not used)
-          weights(s);
+          weights(s, offset);
           const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
 #pragma unroll
           for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
 #pragma unroll
           for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 1, x), p1, o[x]);
-          exponents(n, half + 1 < H ? key0 + 32 : t1 * KT);
+          offset = exponents(n, half + 1 < H ? key0 + 32 : t1 * KT);
           s = n;
         }
         if (half == 0) {
@@ -398,10 +421,10 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
           const bool edge = is_edge(doc, key0);
           f32x16 s;
           scores(s, 0, half);
-          exponents(s, key0);
+          const float offset = exponents(s, key0);
           if (edge) hide(s, key0, 0, half);
-          raise(s);
-          weights(s);
+          raise(s, offset);
+          weights(s, offset);
           if (edge) {
 #pragma unroll 1
             for (int key = 0; key < 32; ++key) {
@@ -410,7 +433,7 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
 #pragma unroll
               for (int y = 0; y < 16; ++y) w = want == y ? s[y] : w;
               w = __shfl(w, c | (key >> 2 & 1) << 5);
-              if (key0 + key >= limit || (td && (ldoc[0][32 * half + key] != qdoc || qdoc < 0))) continue;
+              if (key0 + key >= limit || (td && ldoc[0][32 * half + key] != qdoc)) continue;
 #pragma unroll
               for (int x = 0; x < DB; ++x)
 #pragma unroll
@@ -438,7 +461,10 @@ __global__ __launch_bounds__(512, 2) __attribute__((amdgpu_num_vgpr(256))) void 
 
   l += __shfl_xor(l, 32);
   if (row0 + c >= rows) return;
-  const int64_t row = ((int64_t)b * a.Lq + i) * a.Hq + hq;
+  int group = a.G;
+  asm volatile("" : "+s"(group));                                // (position and head again: not kept in registers through the loop)
+  const int at_i = r / group;
+  const int64_t row = ((int64_t)b * a.Lq + at_i) * a.Hq + kvh * a.G + (r - at_i * group);
   const bool none = m == -INFINITY && l == 0.f;                  // nothing seen: zeros
   if (a.part_o) {
     const int64_t at = (int64_t)part * a.B * a.Lq * a.Hq + row;

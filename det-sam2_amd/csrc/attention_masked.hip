@@ -94,6 +94,7 @@ extern "C" int ds2_op_attention_masked(const ds2_attention_masked_args* args, vo
   a.B = x.B, a.Lq = x.Lq, a.Lk = x.Lk, a.Hq = x.Hq, a.Hkv = x.Hkv, a.G = x.Hq / x.Hkv, a.D = x.D, a.causal = x.causal;
   a.scale = x.scale, a.cap = x.cap;
   a.row_tiles = p.row_tiles, a.heads = p.heads, a.parts = p.parts, a.tiles = p.tiles, a.tiles_a_part = p.tiles_a_part;
+  a.fold = x.causal && x.D <= 64 && p.blocks <= 512;
   hipStream_t st = (hipStream_t)stream;
   if (x.q_doc && p.tiles) {
     int2* docs = (int2*)work;
