@@ -11,12 +11,17 @@ struct AttnJoinArgs {
   char* out;                  // [rows][D], 16 bits
   int64_t rows;
   int D, parts;
-  // caches: parts behind a sequence's last token were not written, and rows before its first token see nothing
-  const int32_t* lens;        // null: all parts count
-  int T, Hq, C, pre_parts, own_chunk;
+  // caches: segments of the row's stream besides (cache_attention.h); rows before a sequence's first token see nothing
+  const float* seg_o;
+  const f32x2_t* seg_ml;
+  const int2* seg_of;
+  const int32_t* lens;        // null: no segments
+  int T, Hq, G, C, own_rows, own_groups;
 };
 
-// WIDE: four waves share the parts of a row (few rows with many parts); otherwise a wave has a row to itself.
+// Latency is what this kernel is made of (2 to 5 us for a few MB): statistics and rows of eight parts are asked for at once and weighed
+// against a running maximum, so a row with up to eight parts (32 in a WIDE one: four waves share the row's parts) waits for memory
+// twice, for where its parts are and for the parts.
 template <bool F16, bool WIDE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
   __shared__ float sum[4][260];
@@ -24,51 +29,67 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
   const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (row >= a.rows) return;
   int parts = a.parts;
+  int64_t seg = 0;                                           // index of part p, p >= a.parts, is seg + p own_rows
   bool none = false;
   if (a.lens) {
-    const int b = (int)(row / ((int64_t)a.T * a.Hq)), t = (int)(row / a.Hq - (int64_t)b * a.T);
+    const int b = (int)(row / ((int64_t)a.T * a.Hq)), rest = (int)(row - (int64_t)b * a.T * a.Hq), t = rest / a.Hq, hq = rest - t * a.Hq;
+    const int head = hq / a.G, r = t * a.G + hq - head * a.G, group = r / a.own_rows;
+    const int stream = (b * (a.Hq / a.G) + head) * a.own_groups + group;
     const int len = max(0, min(a.lens[b], a.C));
-    parts = a.pre_parts + (int)(((int64_t)len + a.own_chunk - 1) / a.own_chunk);
+    const int2 of = a.seg_of[stream];                        // (not written where there is no token)
+    if (len > 0) {
+      parts += of.y - of.x + 1;
+      seg = (int64_t)(of.x + stream - a.parts) * a.own_rows + r - group * a.own_rows;
+    }
     none = len - a.T + t < 0;
   }
   const int first = WIDE ? wave : 0, step = WIDE ? 4 : 1;
-  float m = -INFINITY;
-  for (int p = lane; p < parts; p += 64) m = fmaxf(m, a.ml[p * a.rows + row][0]);
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
   const int d = lane * 4;
   const bool live = d < a.D;
   f32x4 o = {0, 0, 0, 0};
-  float l = 0.f;
-  // four parts at a time: their loads do not wait for one another
-  for (int p = first; p < parts; p += 4 * step) {
-    f32x2_t ml[4];
-    f32x4 x[4];
+  float l = 0.f, m = -INFINITY;
+  for (int p0 = first; p0 < parts; p0 += 8 * step) {
+    f32x2_t ml[8];
+    f32x4 x[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t at = min(p + u * step, parts - 1) * a.rows + row;
-      ml[u] = a.ml[at];
-      x[u] = live ? *(const f32x4*)(a.o + at * a.D + d) : f32x4{0, 0, 0, 0};
+    for (int u = 0; u < 8; ++u) {
+      const int p = min(p0 + u * step, parts - 1);
+      const bool own = p >= a.parts;
+      const int64_t at = own ? seg + (int64_t)p * a.own_rows : p * a.rows + row;
+      ml[u] = (own ? a.seg_ml : a.ml)[at];
+      x[u] = live ? *(const f32x4*)((own ? a.seg_o : a.o) + at * a.D + d) : f32x4{0, 0, 0, 0};
+      if (p0 + u * step >= parts) ml[u] = f32x2_t{-INFINITY, 0.f};
     }
+    float mn = m;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (p + u * step < parts && !(ml[u][0] == -INFINITY && ml[u][1] == 0.f)) {
-        const float f = ml[u][0] == m ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - m);
-        l += f * ml[u][1];
-        o += f * x[u];
+    for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ml[u][0]);
+    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    o *= f, l *= f, m = mn;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (!(ml[u][0] == -INFINITY && ml[u][1] == 0.f)) {     // (a part that saw nothing may not have written its row)
+        const float g = ml[u][0] == m ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - m);
+        l += g * ml[u][1];
+        o += g * x[u];
       }
   }
   if constexpr (WIDE) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[wave][d + j] = o[j];
-    if (lane == 0) sum[wave][256] = l;
+    if (lane == 0) sum[wave][256] = l, sum[wave][257] = m;
     __syncthreads();
     if (wave) return;
+    float mn = m;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) mn = fmaxf(mn, sum[w][257]);
+    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    o *= f, l *= f, m = mn;
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
+      const float g = sum[w][257] == m ? 1.f : __builtin_amdgcn_exp2f(sum[w][257] - m);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += sum[w][d + j];
-      l += sum[w][256];
+      for (int j = 0; j < 4; ++j) o[j] += g * sum[w][d + j];
+      l += g * sum[w][256];
     }
   }
   if (!live) return;
@@ -78,8 +99,9 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
       none ? u32x2{0, 0} : u32x2{ds2_pack16<F16>(o[0] * f, o[1] * f), ds2_pack16<F16>(o[2] * f, o[3] * f)};
 }
 
-inline int launch_attn_join(const AttnJoinArgs& a, bool f16, int most_parts, hipStream_t st) {
-  const bool wide = most_parts > 16;
+// usual_parts: of a row, as far as the host knows; over eight of them four waves share a row
+inline int launch_attn_join(const AttnJoinArgs& a, bool f16, int64_t usual_parts, hipStream_t st) {
+  const bool wide = usual_parts > 8;
   const dim3 grid((unsigned)(wide ? a.rows : cdiv64(a.rows, 4)));
   if (f16) wide ? k_attn_join<true, true><<<grid, 256, 0, st>>>(a) : k_attn_join<true, false><<<grid, 256, 0, st>>>(a);
   else wide ? k_attn_join<false, true><<<grid, 256, 0, st>>>(a) : k_attn_join<false, false><<<grid, 256, 0, st>>>(a);

@@ -26,8 +26,6 @@
 
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
 
@@ -46,6 +44,8 @@ struct MaskedArgs {
   int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;    // bytes
   const float* slopes;
   const int32_t *lens, *q_start, *prefix, *q_doc, *k_doc;
+  const int32_t* row_lens;                  // rows of sequences behind a shared prefix of Lk keys (cache_attention.hip): position i stands at
+  int row_T, row_C;                         // Lk + row_lens[i / row_T] - row_T + i % row_T, row_lens at most row_C; null: at q_start + i
   const int2* tile_docs;                    // [B][tiles]: smallest (-1: a key of none among them) and largest document of a tile
   int B, Lq, Lk, Hq, Hkv, G, D, causal;
   float scale, cap;
@@ -54,6 +54,9 @@ struct MaskedArgs {
   f32x2_t* part_ml;
 };
 
+static inline int masked_mode(float scale, float cap, const float* slopes) {
+  return slopes || (cap == 0.f && !(scale > 0.f)) ? MASKED_SLOPES : cap > 0.f ? MASKED_CAP : MASKED_PLAIN;
+}
 int launch_masked_bf16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
 int launch_masked_f16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
 
@@ -115,7 +118,11 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   const int i = r / a.G, hq = kvh * a.G + (r - i * a.G);
   const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
   const int start = a.q_start ? max(-(1 << 30), min(a.q_start[b], 1 << 30)) : 0;
-  const int pos = start + i;
+  int pos = start + i;
+  if (MODE == MASKED_SLOPES && a.row_lens) {
+    const int seq = i / a.row_T;
+    pos = a.Lk + max(0, min(a.row_lens[seq], a.row_C)) - a.row_T + i - seq * a.row_T;
+  }
   const float slope = MODE == MASKED_SLOPES && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
   int limit = len;
   if (a.causal) {
@@ -247,7 +254,12 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   // exponents up to the bias of the lane's first key, which is returned.
   constexpr bool DOWN = MODE == MASKED_CAP;                      // the largest exponent has the smallest value
   const float factor = MODE == MASKED_PLAIN ? sc : -2.f * cap2;
-  const int pos_first = start + min(row0, rows - 1) / a.G, pos_last = start + min(row0 + 31, rows - 1) / a.G;   // of the wave's rows
+  int pos_first = pos, pos_last = pos;                           // of the wave's rows
+  if constexpr (MODE == MASKED_SLOPES) {
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) pos_first = min(pos_first, __shfl_xor(pos_first, s)), pos_last = max(pos_last, __shfl_xor(pos_last, s));
+    pos_first = __builtin_amdgcn_readfirstlane(pos_first), pos_last = __builtin_amdgcn_readfirstlane(pos_last);
+  }
   auto exponents = [&](f32x16& s, int key0) {
     if constexpr (MODE == MASKED_PLAIN) return 0.f;
     if constexpr (MODE == MASKED_CAP) {

@@ -110,7 +110,7 @@ extern "C" int ds2_op_attention_masked(const ds2_attention_masked_args* args, vo
     a.part_ml = (f32x2_t*)(a.part_o + (int64_t)p.parts * rows * x.D);
   }
   const bool f16 = x.type == DS2_TYPE_F16;
-  const int mode = x.slopes || (x.cap == 0.f && !(x.scale > 0.f)) ? MASKED_SLOPES : x.cap > 0.f ? MASKED_CAP : MASKED_PLAIN;
+  const int mode = masked_mode(x.scale, x.cap, x.slopes);
   if (const int rc = f16 ? launch_masked_f16(a, mode, (unsigned)p.blocks, st) : launch_masked_bf16(a, mode, (unsigned)p.blocks, st)) return rc;
   if (p.parts > 1) {
     AttnJoinArgs j{};

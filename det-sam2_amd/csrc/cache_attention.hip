@@ -4,39 +4,69 @@
 #include <cmath>
 
 #include "attention_join.h"
+#include "attention_masked.h"
 #include "cache_attention.h"
 
 namespace {
 
 struct Split {
-  int own_chunk, own_parts, own_groups, pre_chunk, pre_parts, pre_groups, pre_rows;
-  bool two_tiles;
-  int64_t blocks, pre_blocks;
-  int64_t parts() const { return (int64_t)own_parts + pre_parts; }
+  int shares, own_rows, own_groups, by_rows, pre_chunk, pre_parts, pre_by_rows;
+  bool tiled;                              // the prefix goes to the kernel of whole prompts
+  int pre_row_tiles, pre_tiles;            // its tiles of rows, and of keys a part
+  int64_t streams, blocks, pre_blocks;
+  bool joined() const { return shares || pre_parts; }
+  int64_t segments() const { return shares ? shares + streams : 0; }
 };
-
-int round_up(int64_t x, int to) { return (int)((x + to - 1) / to * to); }
 
 Split split_of(const ds2_cache_attention_args& a) {
   Split s{};
-  const int64_t G = a.Hq / a.Hkv, own_rows = a.T * G, all_rows = a.B * own_rows;
-  // Two tiles of 16 rows a wave where the rows of a call fill them (and a head's 128 values leave the registers for it).
-  s.two_tiles = a.D <= 128 && (own_rows > 16 || (a.prefix_len && all_rows > 16));
-  const int tile = s.two_tiles ? 32 : 16;
-  s.own_groups = (int)cdiv64(own_rows, tile);
-  const int64_t streams = (int64_t)a.B * a.Hkv * s.own_groups;
-  s.own_chunk = std::min(2048, std::max(128, round_up(cdiv64(a.capacity * streams, 2048), 128)));
-  s.own_parts = std::max(1, (int)cdiv64(a.capacity, s.own_chunk));
+  const int64_t G = a.Hq / a.Hkv, rows = a.T * G, all_rows = a.B * rows;
+  s.by_rows = rows > cache_rows(a.D, false);
+  s.own_rows = cache_rows(a.D, s.by_rows);
+  s.own_groups = (int)cdiv64(rows, s.own_rows);
+  s.streams = (int64_t)a.B * a.Hkv * s.own_groups;
+  // Equal shares of all keys, two workgroups a CU (what the registers allow), at least one unit each; caches of a few units a stream
+  // are not worth the second kernel.
+  const int64_t units = cdiv64(a.capacity, CACHE_UNIT) + 1;
+  s.shares = !a.prefix_len && units <= 3 ? 0 : (int)std::min<int64_t>(512, s.streams * units);
   if (a.prefix_len) {
-    s.pre_rows = all_rows > tile;
-    s.pre_groups = (int)cdiv64(all_rows, s.pre_rows ? 4 * tile : tile);
-    const int64_t pre_streams = (int64_t)a.Hkv * s.pre_groups;
-    s.pre_chunk = std::min(2048, std::max(128, round_up(cdiv64(a.prefix_len * pre_streams, 256), 32)));
-    s.pre_parts = (int)cdiv64(a.prefix_len, s.pre_chunk);
-    s.pre_blocks = pre_streams * s.pre_parts;
+    // From 64 rows a key head on, the prefix is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve
+    // 256 rows (16-bit caches whose rows follow each other at one stride).
+    s.tiled = a.format == DS2_CACHE_PLAIN && all_rows >= 64 && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
+    if (s.tiled) {
+      s.pre_row_tiles = (int)cdiv64(all_rows, 256 / masked_value_split(a.D));
+      const int tiles = cdiv(a.prefix_len, masked_tile(a.D));
+      const int64_t whole = (int64_t)a.Hkv * s.pre_row_tiles;
+      s.pre_tiles = (int)std::max<int64_t>(4, cdiv64(tiles * whole, 256));
+      s.pre_parts = cdiv(tiles, s.pre_tiles);
+    } else {
+      s.pre_by_rows = all_rows > cache_rows(a.D, false);
+      const int64_t streams = (int64_t)a.Hkv * cdiv64(all_rows, cache_rows(a.D, s.pre_by_rows));
+      s.pre_chunk = (int)std::min<int64_t>(2048, std::max<int64_t>(CACHE_UNIT, cdiv64(cdiv64(a.prefix_len * streams, 256), CACHE_UNIT) * CACHE_UNIT));
+      s.pre_parts = (int)cdiv64(a.prefix_len, s.pre_chunk);
+      s.pre_blocks = streams * s.pre_parts;
+    }
   }
-  s.blocks = s.pre_blocks + streams * s.own_parts;
+  s.blocks = s.pre_blocks + (s.shares ? s.shares : s.streams);
   return s;
+}
+
+int64_t up16(int64_t x) { return (x + 15) / 16 * 16; }
+
+// the workspace: segments of the sequences' own keys, where a stream's segments are, parts of the prefix
+struct Work {
+  int64_t seg_o, seg_ml, seg_of, pre_o, pre_ml, bytes;
+};
+Work work_of(const ds2_cache_attention_args& a, const Split& s) {
+  Work w{};
+  if (!s.joined()) return w;
+  const int64_t seg = s.segments() * s.own_rows, pre = (int64_t)s.pre_parts * a.B * a.T * a.Hq;
+  w.seg_ml = up16(seg * a.D * 4);
+  w.seg_of = w.seg_ml + up16(seg * 8);
+  w.pre_o = w.seg_of + up16(s.shares ? s.streams * 8 : 0);
+  w.pre_ml = w.pre_o + up16(pre * a.D * 4);
+  w.bytes = w.pre_ml + up16(pre * 8);
+  return w;
 }
 
 int check(const ds2_cache_attention_args& a) {
@@ -48,6 +78,8 @@ int check(const ds2_cache_attention_args& a) {
   DS2_REQUIRE(std::isfinite(a.scale) && std::isfinite(a.cap) && a.cap >= 0.f, "cache_attention: scale and cap must be finite, cap not negative");
   DS2_REQUIRE((int64_t)a.capacity + a.prefix_len < (1ll << 31) - 4096 && a.T < (1 << 20), "cache_attention: too many tokens");
   DS2_REQUIRE((int64_t)a.B * a.T * a.Hq < (1ll << 31) / 256, "cache_attention: too many rows (B T Hq) for one call");
+  const Split s = split_of(a);
+  DS2_REQUIRE(s.blocks < (1ll << 31) && s.streams * (cdiv64(a.capacity, CACHE_UNIT) + 1) < (1ll << 31) - 4096, "cache_attention: too many keys for one call");
   return DS2_OK;
 }
 
@@ -69,9 +101,7 @@ int cache_rows(const ds2_strided& t, int size, int to, const char* name) {
 
 extern "C" int64_t ds2_op_cache_attention_work_bytes(const ds2_cache_attention_args* args) {
   if (!args || check(*args) || !args->B || !args->T) return 0;
-  const Split s = split_of(*args);
-  if (s.parts() <= 1) return 0;
-  return s.parts() * args->B * args->T * args->Hq * ((int64_t)args->D + 2) * 4;
+  return work_of(*args, split_of(*args)).bytes;
 }
 
 extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void* work, int64_t work_bytes, void* stream) {
@@ -107,24 +137,41 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
   a.B = x.B, a.T = x.T, a.Hq = x.Hq, a.Hkv = x.Hkv, a.G = x.Hq / x.Hkv, a.D = x.D, a.C = x.capacity, a.P = x.prefix_len;
   a.scale = x.scale, a.cap = x.cap;
   const Split s = split_of(x);
-  DS2_REQUIRE(s.blocks < (1ll << 31), "cache_attention: too many sequences for one call");
-  a.own_chunk = s.own_chunk, a.own_parts = s.own_parts, a.own_groups = s.own_groups;
-  a.pre_chunk = s.pre_chunk, a.pre_parts = s.pre_parts, a.pre_groups = s.pre_groups, a.pre_rows = s.pre_rows, a.pre_blocks = (int)s.pre_blocks;
-  const int64_t rows = (int64_t)x.B * x.T * x.Hq;
-  if (s.parts() > 1) {
-    DS2_REQUIRE(work && (uintptr_t)work % 16 == 0 && work_bytes >= ds2_op_cache_attention_work_bytes(args), "cache_attention: workspace too small");
-    a.part_o = (float*)work;
-    a.part_ml = (f32x2_t*)(a.part_o + s.parts() * rows * x.D);
+  a.shares = s.shares, a.own_rows = s.own_rows, a.own_groups = s.own_groups, a.by_rows = s.by_rows;
+  a.pre_chunk = s.pre_chunk, a.pre_parts = s.pre_parts, a.pre_by_rows = s.pre_by_rows, a.pre_blocks = (int)s.pre_blocks;
+  if (s.joined()) {
+    const Work w = work_of(x, s);
+    DS2_REQUIRE(work && (uintptr_t)work % 16 == 0 && work_bytes >= w.bytes, "cache_attention: workspace too small");
+    char* p = (char*)work;
+    a.seg_o = (float*)p, a.seg_ml = (f32x2_t*)(p + w.seg_ml), a.seg_of = (int2*)(p + w.seg_of);
+    a.pre_o = (float*)(p + w.pre_o), a.pre_ml = (f32x2_t*)(p + w.pre_ml);
   }
   hipStream_t st = (hipStream_t)stream;
   const bool f16 = x.type == DS2_TYPE_F16;
   const unsigned blocks = (unsigned)s.blocks;
-  DS2_TRY(x.format == DS2_CACHE_PLAIN ? launch_cache_attn_plain(a, f16, s.two_tiles, blocks, st)
-          : x.format == DS2_CACHE_MXFP8 ? launch_cache_attn_mxfp8(a, f16, s.two_tiles, blocks, st)
-                                        : launch_cache_attn_mxfp4(a, f16, s.two_tiles, blocks, st));
-  if (s.parts() > 1) {
-    AttnJoinArgs j{a.part_o, a.part_ml, a.out, rows, x.D, (int)s.parts(), x.lens, x.T, x.Hq, x.capacity, a.pre_parts, a.own_chunk};
-    DS2_TRY(launch_attn_join(j, f16, j.parts, st));
+  if (s.tiled) {
+    MaskedArgs m{};
+    m.q = a.q, m.k = (const char*)a.pk, m.v = (const char*)a.pv, m.out = a.out;
+    m.q_t = x.T == 1 ? a.q_b : a.q_t, m.q_h = a.q_h;
+    m.k_t = a.pk_c, m.k_h = a.pk_h, m.v_t = a.pv_c, m.v_h = a.pv_h;
+    m.slopes = a.slopes, m.row_lens = x.lens, m.row_T = x.T, m.row_C = x.capacity;
+    m.B = 1, m.Lq = x.B * x.T, m.Lk = x.prefix_len, m.Hq = x.Hq, m.Hkv = x.Hkv, m.G = a.G, m.D = x.D;
+    m.scale = x.scale, m.cap = x.cap;
+    m.row_tiles = s.pre_row_tiles, m.heads = x.Hkv, m.parts = s.pre_parts, m.tiles_a_part = s.pre_tiles;
+    m.part_o = a.pre_o, m.part_ml = a.pre_ml;
+    const unsigned tiles = (unsigned)(s.pre_row_tiles * x.Hkv * s.pre_parts);
+    DS2_TRY(f16 ? launch_masked_f16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st) : launch_masked_bf16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st));
+  }
+  DS2_TRY(x.format == DS2_CACHE_PLAIN ? launch_cache_attn_plain(a, f16, blocks, st)
+          : x.format == DS2_CACHE_MXFP8 ? launch_cache_attn_mxfp8(a, f16, blocks, st)
+                                        : launch_cache_attn_mxfp4(a, f16, blocks, st));
+  if (s.joined()) {
+    AttnJoinArgs j{};
+    j.out = a.out, j.rows = (int64_t)x.B * x.T * x.Hq, j.D = x.D;
+    j.o = a.pre_o, j.ml = a.pre_ml, j.parts = a.pre_parts;
+    j.seg_o = a.seg_o, j.seg_ml = a.seg_ml, j.seg_of = a.seg_of, j.lens = x.lens;
+    j.T = x.T, j.Hq = x.Hq, j.G = a.G, j.C = x.capacity, j.own_rows = a.own_rows, j.own_groups = a.own_groups;
+    return launch_attn_join(j, f16, s.pre_parts + std::min<int64_t>(s.shares / s.streams + 2, cdiv64(x.capacity, CACHE_UNIT)), st);
   }
   return DS2_OK;
 }

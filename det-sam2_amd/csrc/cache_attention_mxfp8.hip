@@ -1,6 +1,6 @@
 // Kernels of cache_attention.h for caches in format "mxfp8".
 #include "cache_attention.h"
 
-int launch_cache_attn_mxfp8(const CacheAttnArgs& a, bool f16, bool two_tiles, unsigned blocks, hipStream_t st) {
-  return f16 ? launch_cache_attn_of<DS2_CACHE_MXFP8, true>(a, two_tiles, blocks, st) : launch_cache_attn_of<DS2_CACHE_MXFP8, false>(a, two_tiles, blocks, st);
+int launch_cache_attn_mxfp8(const CacheAttnArgs& a, bool f16, unsigned blocks, hipStream_t st) {
+  return f16 ? launch_cache_attn_of<DS2_CACHE_MXFP8, true>(a, blocks, st) : launch_cache_attn_of<DS2_CACHE_MXFP8, false>(a, blocks, st);
 }
