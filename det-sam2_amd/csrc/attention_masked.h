@@ -133,6 +133,68 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   int qdoc = a.q_doc ? a.q_doc[(int64_t)b * a.Lq + i] : 0;
   qdoc = qdoc < 0 ? -2 : qdoc;                                   // of no document: equal to no key's (a key of none is -1 in LDS)
 
+  // ---- queries
+  u32x4 qf[KS];
+  {
+    const char* row = a.q + b * a.q_b + (int64_t)i * a.q_t + hq * a.q_h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = 16 * s + 8 * h;
+      qf[s] = d < a.D ? *(const u32x4*)(row + d * 2) : u32x4{0, 0, 0, 0};
+    }
+  }
+
+  // ---- staging
+  const int2* td = a.tile_docs ? a.tile_docs + (int64_t)b * a.tiles : nullptr;
+  const char *kb = a.k + b * a.k_b + kvh * a.k_h, *vb = a.v + b * a.v_b + kvh * a.v_h;
+  unsigned k_off[PER], v_off[PER];                               // of the thread's pieces in a tile; beyond any bound where there are none
+  int lds_k[PER], lds_v[PER];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const int p = u * NT + tid, row = p / CH, piece = p - row * CH;
+    const bool place = PER * NT == KT * CH || row < KT, live = place && piece * 8 < a.D;
+    k_off[u] = live ? (unsigned)(row * (int)a.k_t + piece * 16) : 0x80000000u;
+    v_off[u] = live ? (unsigned)(row * (int)a.v_t + piece * 16) : 0x80000000u;
+    lds_k[u] = place ? row * KROW + piece * 16 : KT * KROW, lds_v[u] = place ? row * VROW + piece * 16 : KT * VROW;
+  }
+  struct Tile {
+    u32x4 k[PER], v[PER];
+    int doc;
+  };
+  Tile tile, second;
+  auto fetch = [&](Tile& to, int t) {                            // a tile into registers; behind the last key: zeros
+    const int left = len - t * KT;                               // > 0
+    const int64_t kn = (int64_t)(min(left, KT) - 1) * a.k_t + a.D * 2, vn = (int64_t)(min(left, KT) - 1) * a.v_t + a.D * 2;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (int64_t)t * KT * a.k_t), 0, (int)kn, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (int64_t)t * KT * a.v_t), 0, (int)vn, 0x00020000);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      to.k[u] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[u], 0, 0);
+      to.v[u] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[u], 0, 0);
+    }
+    if (td) {                                                    // (every wave fetches and writes all of the tile's documents: no divergent branch)
+      const __amdgpu_buffer_rsrc_t dr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k_doc + (int64_t)b * a.Lk + t * KT), 0, min(left, KT) * 4, 0x00020000);
+      to.doc = __builtin_amdgcn_raw_buffer_load_b32(dr, lane * 4, 0, 0);
+      to.doc = lane < left ? max(to.doc, -1) : -1;
+    }
+  };
+  auto stage = [&](const Tile& from, int buf) {
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      *(u32x4*)(lk[buf] + lds_k[u]) = from.k[u];
+      *(u32x4*)(lv[buf] + lds_v[u]) = from.v[u];
+    }
+    if (td) ldoc[buf][lane] = from.doc;
+  };
+
+  // The first two tiles of an undocumented call are known before the limits of all rows are: they are asked for at once (a tile behind
+  // every limit is not used).
+  const int t_begin = part * a.tiles_a_part;
+  if (!td && t_begin * KT < len) {
+    fetch(tile, t_begin);
+    if ((t_begin + 1) * KT < len) fetch(second, t_begin + 1);
+  }
+
   // ---- smallest and largest limit and document of the wave and of the workgroup (rows of no document do not widen the range)
   int lo = limit, hi = limit, dlo = qdoc < 0 ? INT32_MAX : qdoc, dhi = qdoc, dmin = qdoc;
 #pragma unroll
@@ -150,10 +212,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   ghi = __builtin_amdgcn_readfirstlane(ghi), gdlo = __builtin_amdgcn_readfirstlane(gdlo), gdhi = __builtin_amdgcn_readfirstlane(gdhi);
 
   const int t_end = min((ghi + KT - 1) / KT, (part + 1) * a.tiles_a_part);
-  const int t_begin = part * a.tiles_a_part;
   // next tile at or behind t that may hold a visible pair (the same answer in every wave); t_end: none.  64 tiles are looked at a time,
   // one a lane, and kept.
-  const int2* td = a.tile_docs ? a.tile_docs + (int64_t)b * a.tiles : nullptr;
   int window = -64;
   unsigned long long window_on = 0;
   int2 mine = {-1, -1};
@@ -176,58 +236,6 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     if (!td || t >= t_end) return -1;
     const int x = __builtin_amdgcn_readlane(mine.x, t - window), y = __builtin_amdgcn_readlane(mine.y, t - window);
     return x == y ? x : -1;
-  };
-
-  // ---- queries
-  u32x4 qf[KS];
-  {
-    const char* row = a.q + b * a.q_b + (int64_t)i * a.q_t + hq * a.q_h;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d = 16 * s + 8 * h;
-      qf[s] = d < a.D ? *(const u32x4*)(row + d * 2) : u32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));  // (arrived here: a wait inside the loop would be for the tile loads too)
-  }
-
-  // ---- staging
-  const char *kb = a.k + b * a.k_b + kvh * a.k_h, *vb = a.v + b * a.v_b + kvh * a.v_h;
-  unsigned k_off[PER], v_off[PER];                               // of the thread's pieces in a tile; beyond any bound where there are none
-  int lds_k[PER], lds_v[PER];
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const int p = u * NT + tid, row = p / CH, piece = p - row * CH;
-    const bool place = PER * NT == KT * CH || row < KT, live = place && piece * 8 < a.D;
-    k_off[u] = live ? (unsigned)(row * (int)a.k_t + piece * 16) : 0x80000000u;
-    v_off[u] = live ? (unsigned)(row * (int)a.v_t + piece * 16) : 0x80000000u;
-    lds_k[u] = place ? row * KROW + piece * 16 : KT * KROW, lds_v[u] = place ? row * VROW + piece * 16 : KT * VROW;
-  }
-  u32x4 sk[PER], sv[PER];
-  int sdoc = -1;
-  auto fetch = [&](int t) {                                      // a tile into registers; behind the last key: zeros
-    const int left = len - t * KT;                               // > 0
-    const int64_t kn = (int64_t)(min(left, KT) - 1) * a.k_t + a.D * 2, vn = (int64_t)(min(left, KT) - 1) * a.v_t + a.D * 2;
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (int64_t)t * KT * a.k_t), 0, (int)kn, 0x00020000);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (int64_t)t * KT * a.v_t), 0, (int)vn, 0x00020000);
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      sk[u] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off[u], 0, 0);
-      sv[u] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off[u], 0, 0);
-    }
-    if (td) {                                                    // (every wave fetches and writes all of the tile's documents: no divergent branch)
-      const __amdgpu_buffer_rsrc_t dr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k_doc + (int64_t)b * a.Lk + t * KT), 0, min(left, KT) * 4, 0x00020000);
-      sdoc = __builtin_amdgcn_raw_buffer_load_b32(dr, lane * 4, 0, 0);
-      sdoc = lane < left ? max(sdoc, -1) : -1;
-    }
-  };
-  auto stage = [&](int buf) {
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      *(u32x4*)(lk[buf] + lds_k[u]) = sk[u];
-      *(u32x4*)(lv[buf] + lds_v[u]) = sv[u];
-    }
-    if (td) ldoc[buf][lane] = sdoc;
   };
 
   // ---- pieces of a step
@@ -354,13 +362,15 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   int t0 = next_tile(t_begin), doc0 = tile_doc(t0);
   if (t0 < t_end) {
     int t1 = next_tile(t0 + 1), doc1 = tile_doc(t1), t2 = next_tile(t1 + 1), doc2 = tile_doc(t2), t3 = t_end, doc3 = -1, buf = 0;
-    fetch(t0);
-    stage(0);
-    if (t1 < t_end) {
-      fetch(t1);
-      stage(1);
+    if (td) {
+      fetch(tile, t0);
+      if (t1 < t_end) fetch(second, t1);
     }
-    if (t2 < t_end) fetch(t2);
+    stage(tile, 0);
+    if (t1 < t_end) stage(second, 1);
+    if (t2 < t_end) fetch(tile, t2);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s])); // (arrived before the loop: a wait inside it would be for the tile loads too)
     __syncthreads();
     f32x16 s;
     scores(s, 0, 0);
@@ -390,9 +400,9 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           s = n;
         }
         if (half == 0) {
-          if (t2 < t_end) stage(next == 2 ? 0 : next + 1);       // (that buffer was last read before this tile's barrier)
+          if (t2 < t_end) stage(tile, next == 2 ? 0 : next + 1);       // (that buffer was last read before this tile's barrier)
           t3 = next_tile(t2 + 1), doc3 = tile_doc(t3);
-          if (t3 < t_end) fetch(t3);
+          if (t3 < t_end) fetch(tile, t3);
         }
       }
       if (t1 >= t_end) break;
@@ -423,8 +433,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
       for (int t = next_tile(t_begin); t < t_end; t = next_tile(t + 1)) {
         const int doc = tile_doc(t);
         __syncthreads();
-        fetch(t);
-        stage(0);
+        fetch(tile, t);
+        stage(tile, 0);
         __syncthreads();
 #pragma unroll 1
         for (int half = 0; half < H; ++half) {

@@ -159,34 +159,36 @@ struct CacheStream {
 
   __device__ __forceinline__ void start(const char* row, bool live, int g) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      u32x4 w = {0, 0, 0, 0};
-      if (live) w = *(const u32x4*)(row + (g * KS + s) * 16);
-      if constexpr (QLO) {
-        u32x4 hi, lo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = ds2_low16<true>(w[j]), y = ds2_high16<true>(w[j]);
-          hi[j] = ds2_pack16<false>(x, y);
-          lo[j] = ds2_pack16<false>(x - ds2_low16<false>(hi[j]), y - ds2_high16<false>(hi[j]));
-          // (an infinite query has no remainder: inf - inf would be NaN)
-          lo[j] &= ~ds2_not_finite16<false>(lo[j]);
-        }
-        q[s] = hi, ql[s] = lo;
-      } else q[s] = w;
-    }
+    for (int s = 0; s < KS; ++s) q[s] = live ? *(const u32x4*)(row + (g * KS + s) * 16) : u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < E; ++t) o[t] = f32x4{0, 0, 0, 0};
     m = -INFINITY, l = 0.f;
   }
+  // fp16 queries as the sum of two bf16 operands
+  __device__ __forceinline__ void split_queries() {
+    if constexpr (QLO) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = ds2_low16<true>(q[s][j]), y = ds2_high16<true>(q[s][j]);
+          const unsigned hi = ds2_pack16<false>(x, y), lo = ds2_pack16<false>(x - ds2_low16<false>(hi), y - ds2_high16<false>(hi));
+          q[s][j] = hi, ql[s][j] = lo & ~ds2_not_finite16<false>(lo);     // (an infinite query has no remainder: inf - inf would be NaN)
+        }
+    }
+  }
 
   // 32 keys to the wave's LDS (rows behind the end: whatever is there, their scores are replaced) and their scales to registers
+  // (`stride` and `scale_stride` pass through an empty asm statement: offsets made from them are an addition a load, not two dozen
+  // registers kept through the loop)
   __device__ __forceinline__ void load_keys(const CacheRows& c, int blk, int k1, unsigned char* lds, int lane) {
+    unsigned stride = c.k_c, scale_stride = c.ks_c;
+    asm volatile("" : "+s"(stride), "+s"(scale_stride));
     const __amdgpu_buffer_rsrc_t r = ds2_rows(c.k, blk, c.k_c, k1 - blk, ROW);
 #pragma unroll
     for (int n = 0; n < ISSUES; ++n) {
       const int p = n * 64 + lane, row = p / PIECES;
-      const unsigned at = PIECES * 32 % 64 && p >= PIECES * 32 ? 0x80000000u : row * c.k_c + mixed(row, p - row * PIECES) * 16;
+      const unsigned at = PIECES * 32 % 64 && p >= PIECES * 32 ? 0x80000000u : row * stride + mixed(row, p - row * PIECES) * 16;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + n * 1024), 16, at, 0, 0, 0);
     }
     if constexpr (QUANT) {
@@ -196,7 +198,7 @@ struct CacheStream {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int x = 0; x < SG; ++x)
-          kscale[t][x] = __builtin_amdgcn_raw_buffer_load_b8(rs, (16 * t + i) * c.ks_c + ((KS == 3 ? g * 3 + x : g * KS + 4 * x) >> 2), 0, 0);
+          kscale[t][x] = __builtin_amdgcn_raw_buffer_load_b8(rs, (16 * t + i) * scale_stride + ((KS == 3 ? g * 3 + x : g * KS + 4 * x) >> 2), 0, 0);
     }
   }
   // Loads to LDS are not followed by hipcc: the reads wait for them here.  Loads return in order and the block's value loads were asked
@@ -222,13 +224,16 @@ struct CacheStream {
     }
   }
   __device__ __forceinline__ void load_values(const CacheRows& c, int blk, int k1, unsigned v_lane, unsigned vs_lane, int g) {
+    unsigned stride = c.v_c, scale_stride = c.vs_c;
+    asm volatile("" : "+s"(stride), "+s"(scale_stride));
     const __amdgpu_buffer_rsrc_t r = ds2_rows(c.v, blk, c.v_c, k1 - blk, ROW);
     const __amdgpu_buffer_rsrc_t rs = ds2_rows(c.vs, blk, c.vs_c, k1 - blk, KS);
+    const unsigned first = 4 * g * stride + v_lane, scale_first = 4 * g * scale_stride + vs_lane;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const unsigned row = (j < 4 ? 0 : 12) + 4 * g + j;
-      ds2_load_bytes<VB>(vw[j], r, row * c.v_c + v_lane);
-      if constexpr (QUANT) vscale[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, row * c.vs_c + vs_lane, 0, 0);
+      const unsigned row = (j < 4 ? 0 : 12) + j;           // + 4 g
+      ds2_load_bytes<VB>(vw[j], r, first + row * stride);
+      if constexpr (QUANT) vscale[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, scale_first + row * scale_stride, 0, 0);
     }
   }
 
@@ -246,6 +251,7 @@ struct CacheStream {
     load_keys(c, blk, k1, lds, lane);
     asm volatile("" ::: "memory");                         // (keys before values: wait_keys counts on it)
     load_values(c, blk, k1, v_lane, vs_lane, g);
+    split_queries();                                       // (after the loads have been asked for)
     for (; blk < k1; blk += step * 32) {
       const int next = blk + step * 32;
       // ---- scores
@@ -394,9 +400,11 @@ constexpr int cache_value_split(int D) { return D > 128 ? 2 : 1; }
 // rows of a workgroup: its waves share 16 rows and split the keys, or each holds 16 rows of its own over the same keys
 constexpr int cache_rows(int D, bool by_rows) { return by_rows ? 4 / cache_value_split(D) * 16 : 16; }
 
-// (no accumulators in AGPRs: hipcc has left out wait states in front of their reads)
+// workgroups (and waves a SIMD) that a CU holds, by registers; the shares of the keys are as many as fit the chip
+constexpr int cache_residents(int D) { return D > 128 ? 2 : D > 64 ? 3 : 4; }
+
 template <int FORMAT, bool QF16, int KS, int E, int VS>
-__global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void k_cache_attn(CacheAttnArgs a) {
+__global__ __launch_bounds__(256, cache_residents(32 * KS)) void k_cache_attn(CacheAttnArgs a) {
   typedef CacheStream<FORMAT, QF16, KS, E, VS> Stream;
   constexpr bool FULL = Stream::FULL;
   constexpr int KW = 4 / VS;                               // waves of a workgroup that share its keys (or hold different rows)
@@ -413,10 +421,9 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void 
   const int heads = a.Hkv * a.own_groups;                  // streams of a sequence
   int part = 0, head = 0, group = 0, b = 0, at = 0, end = 1, base = 0, units = 1;
   const int share = blockIdx.x - a.pre_blocks;
-  auto units_of = [&](int x) {                             // and one for its beginning
-    const int n = max(0, min(a.lens[x], a.C));
-    return n ? (n + CACHE_UNIT - 1) / CACHE_UNIT + 1 : 0;
-  };
+  const int len0 = lane < a.B ? max(0, min(a.lens[lane], a.C)) : 0;        // of the first 64 sequences, kept
+  auto len_of = [&](int x) { return x < 64 ? __builtin_amdgcn_readlane(len0, x) : max(0, min(a.lens[x], a.C)); };
+  auto units_of = [&](int n) { return n ? (n + CACHE_UNIT - 1) / CACHE_UNIT + 1 : 0; };                  // one for the stream's beginning
   if (prefix) {                                            // row groups over the same keys are far apart in id: same chiplet, one L2
     int id = blockIdx.x;
     group = id / (a.Hkv * a.pre_parts), id -= group * a.Hkv * a.pre_parts;
@@ -424,15 +431,15 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void 
   } else if (a.shares == 0) {
     b = share / heads;
   } else {
-    int sum = 0;
-    for (int x = lane; x < a.B; x += 64) sum += units_of(x);
+    int sum = units_of(len0);
+    for (int x = lane + 64; x < a.B; x += 64) sum += units_of(max(0, min(a.lens[x], a.C)));
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
     const int total = __builtin_amdgcn_readfirstlane(sum) * heads, each = max(1, (total + a.shares - 1) / a.shares);
     at = share * each, end = min(total, at + each);
     if (at >= end) return;
     for (int b0 = 0;; b0 += 64) {                          // the sequence in which the share begins
-      int x = b0 + lane < a.B ? units_of(b0 + lane) * heads : 0;
+      int x = (b0 == 0 ? units_of(len0) : b0 + lane < a.B ? units_of(max(0, min(a.lens[b0 + lane], a.C))) : 0) * heads;
       const int mine = x;
 #pragma unroll
       for (int s = 1; s < 64; s <<= 1) {
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void 
     if (prefix) {
       len = a.P, k0 = part * a.pre_chunk, k1 = min(len, k0 + a.pre_chunk);
     } else {
-      len = max(0, min(a.lens[b], a.C));
+      len = len_of(b);
       if (a.shares == 0) hg = share - b * heads, k0 = 0, k1 = len;
       else {
         hg = (at - base) / units;
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(256, 2) __attribute__((amdgpu_num_vgpr(256))) void 
     if (!by_rows) __syncthreads();                         // (what the waves handed over has been read)
     while (at >= base + units * heads) {                   // the next sequence that holds tokens
       base += units * heads;
-      units = __builtin_amdgcn_readfirstlane(units_of(++b));
+      units = units_of(len_of(++b));
     }
   }
 }

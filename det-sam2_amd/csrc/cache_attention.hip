@@ -25,10 +25,10 @@ Split split_of(const ds2_cache_attention_args& a) {
   s.own_rows = cache_rows(a.D, s.by_rows);
   s.own_groups = (int)cdiv64(rows, s.own_rows);
   s.streams = (int64_t)a.B * a.Hkv * s.own_groups;
-  // Equal shares of all keys, two workgroups a CU (what the registers allow), at least one unit each; caches of a few units a stream
-  // are not worth the second kernel.
+  // Equal shares of all keys, as many as the chip holds workgroups, at least one unit each; caches of a few units a stream are not
+  // worth the second kernel.
   const int64_t units = cdiv64(a.capacity, CACHE_UNIT) + 1;
-  s.shares = !a.prefix_len && units <= 3 ? 0 : (int)std::min<int64_t>(512, s.streams * units);
+  s.shares = !a.prefix_len && units <= 3 ? 0 : (int)std::min<int64_t>(256 * cache_residents(a.D), s.streams * units);
   if (a.prefix_len) {
     // From 64 rows a key head on, the prefix is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve
     // 256 rows (16-bit caches whose rows follow each other at one stride).
