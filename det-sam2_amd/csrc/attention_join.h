@@ -16,15 +16,19 @@ struct AttnJoinArgs {
   const f32x2_t* seg_ml;
   const int2* seg_of;
   const int32_t* lens;        // null: no segments
-  int T, Hq, G, C, own_rows, own_groups;
+  int T, Hq, G, C, shares, own_rows, own_groups;
+  int lanes;                  // of a reader, set at the launch
 };
 
-// Latency is what this kernel is made of (2 to 5 us for a few MB): statistics and rows of eight parts are asked for at once and weighed
-// against a running maximum, so a row with up to eight parts (32 in a WIDE one: four waves share the row's parts) waits for memory
-// twice, for where its parts are and for the parts.
+// Latency is what this kernel is made of (2 to 5 us for a few MB), so little of it is one after the other: D / 4 lanes (rounded up
+// to a power of two) are a reader of parts, a wave holds 64 / that many readers, WIDE four times as many (a row for the workgroup's
+// four waves); every reader asks for statistics and rows of eight parts at once and weighs them against a running maximum.  A row of
+// up to eight parts a reader waits for memory twice: for where its parts are, and for the parts.
+inline int attn_join_lanes(int D) { return D <= 32 ? 8 : D <= 64 ? 16 : D <= 128 ? 32 : 64; }
+
 template <bool F16, bool WIDE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
-  __shared__ float sum[4][260];
+  __shared__ __attribute__((aligned(16))) float sum[3][260];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (row >= a.rows) return;
@@ -36,18 +40,28 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
     const int head = hq / a.G, r = t * a.G + hq - head * a.G, group = r / a.own_rows;
     const int stream = (b * (a.Hq / a.G) + head) * a.own_groups + group;
     const int len = max(0, min(a.lens[b], a.C));
-    const int2 of = a.seg_of[stream];                        // (not written where there is no token)
+    const int2 of = a.shares ? a.seg_of[stream] : int2{0, 0};       // (not written where there is no token)
     if (len > 0) {
       parts += of.y - of.x + 1;
       seg = (int64_t)(of.x + stream - a.parts) * a.own_rows + r - group * a.own_rows;
     }
     none = len - a.T + t < 0;
   }
-  const int first = WIDE ? wave : 0, step = WIDE ? 4 : 1;
-  const int d = lane * 4;
+  const int each = a.lanes, readers = 64 / each;
+  const int first = (WIDE ? wave * readers : 0) + lane / each, step = (WIDE ? 4 : 1) * readers;
+  const int d = (lane & (each - 1)) * 4;
   const bool live = d < a.D;
   f32x4 o = {0, 0, 0, 0};
   float l = 0.f, m = -INFINITY;
+  auto add = [&](float mp, float lp, f32x4 op) {             // (one part, m is not below mp)
+    const float g = mp == m ? 1.f : __builtin_amdgcn_exp2f(mp - m);
+    l += g * lp;
+    o += g * op;
+  };
+  auto raise = [&](float mn) {
+    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    o *= f, l *= f, m = mn;
+  };
   for (int p0 = first; p0 < parts; p0 += 8 * step) {
     f32x2_t ml[8];
     f32x4 x[8];
@@ -63,45 +77,41 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
     float mn = m;
 #pragma unroll
     for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ml[u][0]);
-    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    o *= f, l *= f, m = mn;
+    raise(mn);
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (!(ml[u][0] == -INFINITY && ml[u][1] == 0.f)) {     // (a part that saw nothing may not have written its row)
-        const float g = ml[u][0] == m ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - m);
-        l += g * ml[u][1];
-        o += g * x[u];
-      }
+      if (!(ml[u][0] == -INFINITY && ml[u][1] == 0.f)) add(ml[u][0], ml[u][1], x[u]);    // (a part that saw nothing may not have written its row)
+  }
+  for (int s = each; s < 64; s <<= 1) {                      // the wave's readers
+    const float mo = __shfl_xor(m, s), lo = __shfl_xor(l, s);
+    const f32x4 oo = {__shfl_xor(o[0], s), __shfl_xor(o[1], s), __shfl_xor(o[2], s), __shfl_xor(o[3], s)};
+    raise(fmaxf(m, mo));
+    add(mo, lo, oo);
   }
   if constexpr (WIDE) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[wave][d + j] = o[j];
-    if (lane == 0) sum[wave][256] = l, sum[wave][257] = m;
+    if (wave && lane < each) {
+      *(f32x4*)&sum[wave - 1][d] = o;
+      if (lane == 0) sum[wave - 1][256] = l, sum[wave - 1][257] = m;
+    }
     __syncthreads();
     if (wave) return;
-    float mn = m;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) mn = fmaxf(mn, sum[w][257]);
-    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    o *= f, l *= f, m = mn;
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float g = sum[w][257] == m ? 1.f : __builtin_amdgcn_exp2f(sum[w][257] - m);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += g * sum[w][d + j];
-      l += g * sum[w][256];
+    for (int w = 0; w < 3; ++w) {
+      raise(fmaxf(m, sum[w][257]));
+      add(sum[w][257], sum[w][256], *(const f32x4*)&sum[w][d]);
     }
   }
-  if (!live) return;
+  if (!live || lane >= each) return;
   none |= m == -INFINITY && l == 0.f;                        // nothing seen: zeros
   const float f = 1.f / l;
   *(u32x2*)(a.out + (row * a.D + d) * 2) =
       none ? u32x2{0, 0} : u32x2{ds2_pack16<F16>(o[0] * f, o[1] * f), ds2_pack16<F16>(o[2] * f, o[3] * f)};
 }
 
-// usual_parts: of a row, as far as the host knows; over eight of them four waves share a row
-inline int launch_attn_join(const AttnJoinArgs& a, bool f16, int64_t usual_parts, hipStream_t st) {
-  const bool wide = usual_parts > 8;
+// usual_parts: of a row, as far as the host knows; over eight of them a reader, four waves share a row
+inline int launch_attn_join(AttnJoinArgs a, bool f16, int64_t usual_parts, hipStream_t st) {
+  a.lanes = attn_join_lanes(a.D);
+  const bool wide = usual_parts > 8 * (64 / a.lanes);
   const dim3 grid((unsigned)(wide ? a.rows : cdiv64(a.rows, 4)));
   if (f16) wide ? k_attn_join<true, true><<<grid, 256, 0, st>>>(a) : k_attn_join<true, false><<<grid, 256, 0, st>>>(a);
   else wide ? k_attn_join<false, true><<<grid, 256, 0, st>>>(a) : k_attn_join<false, false><<<grid, 256, 0, st>>>(a);

@@ -50,12 +50,13 @@ struct CacheAttnArgs {
   const float* slopes;
   int B, T, Hq, Hkv, G, D, C, P;
   float scale, cap;
-  int shares;                              // workgroups that share the sequences' own keys; 0: one workgroup a stream, results written at once
+  int shares;                              // workgroups that share the sequences' own keys; 0: one workgroup a stream
+  bool direct;                             // ... and nothing to join: results are written at once
   int own_rows, own_groups;                // rows of a workgroup, row groups of a key head
   int pre_chunk, pre_parts;                // prefix keys of a workgroup, parts
   int pre_blocks;                          // workgroups [0, pre_blocks) work on the prefix
   int by_rows, pre_by_rows;                // the waves of a workgroup hold different rows over the same keys, or the same rows and different keys
-  float* seg_o;                            // [shares + streams][own_rows][D]: segment share + stream
+  float* seg_o;                            // [shares + streams][own_rows][D]: segment share + stream (stream, where shares is 0)
   f32x2_t* seg_ml;                         // [shares + streams][own_rows]
   int2* seg_of;                            // [streams]: first and last share of a stream
   float* pre_o;                            // [pre_parts][B T Hq][D]
@@ -538,8 +539,8 @@ __global__ __launch_bounds__(256, cache_residents(32 * KS)) void k_cache_attn(Ca
         float l = st.l;
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if (live && (prefix || a.shares)) {
-          const int64_t to = prefix ? (int64_t)part * a.B * a.T * a.Hq + row_id : (int64_t)(share + stream) * a.own_rows + own_row;
+        if (live && (prefix || !a.direct)) {
+          const int64_t to = prefix ? (int64_t)part * a.B * a.T * a.Hq + row_id : (int64_t)((a.shares ? share : 0) + stream) * a.own_rows + own_row;
           if (g == 0 && vh == 0) (prefix ? a.pre_ml : a.seg_ml)[to] = f32x2_t{st.m, l};
           float* out = (prefix ? a.pre_o : a.seg_o) + to * Stream::D;
 #pragma unroll

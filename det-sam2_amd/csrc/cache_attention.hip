@@ -15,7 +15,7 @@ struct Split {
   int pre_row_tiles, pre_tiles;            // its tiles of rows, and of keys a part
   int64_t streams, blocks, pre_blocks;
   bool joined() const { return shares || pre_parts; }
-  int64_t segments() const { return shares ? shares + streams : 0; }
+  int64_t segments() const { return joined() ? shares + streams : 0; }
 };
 
 Split split_of(const ds2_cache_attention_args& a) {
@@ -25,10 +25,13 @@ Split split_of(const ds2_cache_attention_args& a) {
   s.own_rows = cache_rows(a.D, s.by_rows);
   s.own_groups = (int)cdiv64(rows, s.own_rows);
   s.streams = (int64_t)a.B * a.Hkv * s.own_groups;
-  // Equal shares of all keys, as many as the chip holds workgroups, at least one unit each; caches of a few units a stream are not
-  // worth the second kernel.
-  const int64_t units = cdiv64(a.capacity, CACHE_UNIT) + 1;
-  s.shares = !a.prefix_len && units <= 3 ? 0 : (int)std::min<int64_t>(256 * cache_residents(a.D), s.streams * units);
+  // A workgroup for every stream, or equal shares of all keys, as many as the chip holds workgroups.  Streams of one unit or two are not
+  // worth the join; the more streams there are, the less the longest one stands out and the longer a stream may be (uniform 8-bit
+  // D = 128, a workgroup a stream against shares: 64 streams of 512 keys 13.3 / 16.5 us, of 1024 17.4 / 18.0 and ragged 17.9 / 15.9;
+  // 256 streams of 1024 22.1 / 25.5; 1024 of 2048 98.5 / 114).
+  const int64_t units = cdiv64(a.capacity, CACHE_UNIT);
+  const bool whole = units <= std::max<int64_t>(4, std::min<int64_t>(16, s.streams / 32));
+  s.shares = whole ? 0 : (int)std::min<int64_t>(256 * cache_residents(a.D), s.streams * (units + 1));
   if (a.prefix_len) {
     // From 64 rows a key head on, the prefix is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve
     // 256 rows (16-bit caches whose rows follow each other at one stride).
@@ -37,7 +40,7 @@ Split split_of(const ds2_cache_attention_args& a) {
       s.pre_row_tiles = (int)cdiv64(all_rows, 256 / masked_value_split(a.D));
       const int tiles = cdiv(a.prefix_len, masked_tile(a.D));
       const int64_t whole = (int64_t)a.Hkv * s.pre_row_tiles;
-      s.pre_tiles = (int)std::max<int64_t>(4, cdiv64(tiles * whole, 256));
+      s.pre_tiles = (int)std::max<int64_t>(a.D <= 64 ? 8 : 4, cdiv64(tiles * whole, 256));
       s.pre_parts = cdiv(tiles, s.pre_tiles);
     } else {
       s.pre_by_rows = all_rows > cache_rows(a.D, false);
@@ -137,7 +140,7 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
   a.B = x.B, a.T = x.T, a.Hq = x.Hq, a.Hkv = x.Hkv, a.G = x.Hq / x.Hkv, a.D = x.D, a.C = x.capacity, a.P = x.prefix_len;
   a.scale = x.scale, a.cap = x.cap;
   const Split s = split_of(x);
-  a.shares = s.shares, a.own_rows = s.own_rows, a.own_groups = s.own_groups, a.by_rows = s.by_rows;
+  a.shares = s.shares, a.direct = !s.joined(), a.own_rows = s.own_rows, a.own_groups = s.own_groups, a.by_rows = s.by_rows;
   a.pre_chunk = s.pre_chunk, a.pre_parts = s.pre_parts, a.pre_by_rows = s.pre_by_rows, a.pre_blocks = (int)s.pre_blocks;
   if (s.joined()) {
     const Work w = work_of(x, s);
@@ -170,8 +173,8 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
     j.out = a.out, j.rows = (int64_t)x.B * x.T * x.Hq, j.D = x.D;
     j.o = a.pre_o, j.ml = a.pre_ml, j.parts = a.pre_parts;
     j.seg_o = a.seg_o, j.seg_ml = a.seg_ml, j.seg_of = a.seg_of, j.lens = x.lens;
-    j.T = x.T, j.Hq = x.Hq, j.G = a.G, j.C = x.capacity, j.own_rows = a.own_rows, j.own_groups = a.own_groups;
-    return launch_attn_join(j, f16, s.pre_parts + std::min<int64_t>(s.shares / s.streams + 2, cdiv64(x.capacity, CACHE_UNIT)), st);
+    j.T = x.T, j.Hq = x.Hq, j.G = a.G, j.C = x.capacity, j.shares = a.shares, j.own_rows = a.own_rows, j.own_groups = a.own_groups;
+    return launch_attn_join(j, f16, s.pre_parts + std::min<int64_t>(s.shares / s.streams + (s.shares ? 2 : 1), cdiv64(x.capacity, CACHE_UNIT)), st);
   }
   return DS2_OK;
 }
