@@ -34,7 +34,9 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
 constexpr int masked_value_split(int D) { return D > 128 ? 2 : 1; }
 constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }     // keys of a tile
 constexpr float LOG2E = 1.44269504088896340736f;
-enum { MASKED_PLAIN = 0, MASKED_CAP = 1, MASKED_SLOPES = 2 };      // how scores become exponents (SLOPES: cap too, if it is set)
+// How scores become exponents.  LINEAR: distance bias without a cap; GENERAL: both, or a scale that the others do not take.  (With a
+// cap that is decided at run time hipcc computed the tanh always and selected: 1.26 us a step instead of 0.89.)
+enum { MASKED_PLAIN = 0, MASKED_CAP = 1, MASKED_LINEAR = 2, MASKED_GENERAL = 3 };
 
 }  // namespace
 
@@ -55,7 +57,9 @@ struct MaskedArgs {
 };
 
 static inline int masked_mode(float scale, float cap, const float* slopes) {
-  return slopes || (cap == 0.f && !(scale > 0.f)) ? MASKED_SLOPES : cap > 0.f ? MASKED_CAP : MASKED_PLAIN;
+  if (cap > 0.f) return slopes ? MASKED_GENERAL : MASKED_CAP;
+  if (!(scale >= 0x1p-60f)) return MASKED_GENERAL;               // (PLAIN needs a positive scale, LINEAR divides by it)
+  return slopes ? MASKED_LINEAR : MASKED_PLAIN;
 }
 int launch_masked_bf16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
 int launch_masked_f16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
@@ -81,6 +85,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   constexpr int NW = 8;                                          // waves (those without rows of their own stage keys for the others)
   constexpr int KT = masked_tile(DP), H = KT / 32;               // steps of a tile
   constexpr int VS = masked_value_split(DP), RW = NW / VS;       // waves that share rows (each takes 1 / VS of the output), waves of other rows
+  constexpr bool BIAS = MODE >= MASKED_LINEAR;
   constexpr int KS = DP / 16, DB = DP / 32 / VS;                 // contraction steps of a score, a wave's blocks of 32 output elements
   constexpr int KROW = DP * 2 + 16, VROW = DP == 32 ? 64 : DP == 64 ? 192 : DP == 96 ? 192 : DP == 128 ? 320 : 576;
   constexpr int CH = DP / 8;                                     // 16-byte pieces of a row
@@ -119,11 +124,11 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
   const int start = a.q_start ? max(-(1 << 30), min(a.q_start[b], 1 << 30)) : 0;
   int pos = start + i;
-  if (MODE == MASKED_SLOPES && a.row_lens) {
+  if (BIAS && a.row_lens) {
     const int seq = i / a.row_T;
     pos = a.Lk + max(0, min(a.row_lens[seq], a.row_C)) - a.row_T + i - seq * a.row_T;
   }
-  const float slope = MODE == MASKED_SLOPES && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
+  float slope = BIAS && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
   int limit = len;
   if (a.causal) {
     int n = pos + 1;
@@ -159,7 +164,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   }
   struct Tile {
     u32x4 k[PER], v[PER];
-    int doc;
+    int doc, left;                                               // left: keys from the tile's first one on
   };
   Tile tile, second;
   auto fetch = [&](Tile& to, int t) {                            // a tile into registers; behind the last key: zeros
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     if (td) {                                                    // (every wave fetches and writes all of the tile's documents: no divergent branch)
       const __amdgpu_buffer_rsrc_t dr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k_doc + (int64_t)b * a.Lk + t * KT), 0, min(left, KT) * 4, 0x00020000);
       to.doc = __builtin_amdgcn_raw_buffer_load_b32(dr, lane * 4, 0, 0);
-      to.doc = lane < left ? max(to.doc, -1) : -1;
+      to.left = left;
     }
   };
   auto stage = [&](const Tile& from, int buf) {
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
       *(u32x4*)(lk[buf] + lds_k[u]) = from.k[u];
       *(u32x4*)(lv[buf] + lds_v[u]) = from.v[u];
     }
-    if (td) ldoc[buf][lane] = from.doc;
+    if (td) ldoc[buf][lane] = lane < from.left ? max(from.doc, -1) : -1;
   };
 
   // The first two tiles of an undocumented call are known before the limits of all rows are: they are asked for at once (a tile behind
@@ -202,7 +207,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s)), dmin = min(dmin, __shfl_xor(dmin, s));
     dlo = min(dlo, __shfl_xor(dlo, s)), dhi = max(dhi, __shfl_xor(dhi, s));
   }
-  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi), dlo = __builtin_amdgcn_readfirstlane(dlo);
   dmin = __builtin_amdgcn_readfirstlane(dmin), dhi = __builtin_amdgcn_readfirstlane(dhi);
   if (lane == 0) wg_lim[wave][1] = hi, wg_lim[wave][2] = dlo, wg_lim[wave][3] = dhi;
   __syncthreads();
@@ -231,11 +236,12 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     }
     return t_end;
   };
-  // the one document of the tile that next_tile has just found; -1: several, or keys of none
+  // the one document of the tile that next_tile has just found; -1: several, or keys of none; OTHER: none of the wave's rows
+  constexpr int OTHER = -2;
   auto tile_doc = [&](int t) {
     if (!td || t >= t_end) return -1;
     const int x = __builtin_amdgcn_readlane(mine.x, t - window), y = __builtin_amdgcn_readlane(mine.y, t - window);
-    return x == y ? x : -1;
+    return x > dhi || y < dlo ? OTHER : x == y ? x : -1;
   };
 
   // ---- pieces of a step
@@ -251,50 +257,65 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
       for (int y = 0; y < 16; ++y) o[x][y] = 0.f;
     m = -INFINITY, l = 0.f;
   };
-  auto scores = [&](f32x16& s, int buf, int half) {
-#pragma unroll
-    for (int y = 0; y < 16; ++y) s[y] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mfma32<F16>(*(const u32x4*)(lk[buf] + half * 32 * KROW + k_lane + ks * 32), qf[ks], s);
-  };
-  // scores -> values whose exponent (base 2) is factor * value + offset: PLAIN the scores themselves; CAP 1 / (1 + exp(2 x / cap)), as
-  // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)) (no branch, saturates by itself; off by a few 2^-24 of cap); SLOPES
-  // exponents up to the bias of the lane's first key, which is returned.
-  constexpr bool DOWN = MODE == MASKED_CAP;                      // the largest exponent has the smallest value
-  const float factor = MODE == MASKED_PLAIN ? sc : -2.f * cap2;
   int pos_first = pos, pos_last = pos;                           // of the wave's rows
-  if constexpr (MODE == MASKED_SLOPES) {
+  float tilt = 0.f;
+  if constexpr (BIAS) {
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) pos_first = min(pos_first, __shfl_xor(pos_first, s)), pos_last = max(pos_last, __shfl_xor(pos_last, s));
     pos_first = __builtin_amdgcn_readfirstlane(pos_first), pos_last = __builtin_amdgcn_readfirstlane(pos_last);
+    // (a bias of 2^40 a token leaves the nearest key alone like any larger one: no division overflows)
+    if constexpr (MODE == MASKED_LINEAR) slope = fmaxf(-0x1p100f * sc, fminf(slope, 0x1p100f * sc)), tilt = slope / sc;
   }
-  auto exponents = [&](f32x16& s, int key0) {
-    if constexpr (MODE == MASKED_PLAIN) return 0.f;
+  // Scores of the 32 keys from key0 on.  LINEAR: the products are added to the bias over the scale, up to the bias of the lane's first
+  // key, which is returned: where all keys lie on one side of all rows the bias is linear in the key.
+  auto scores = [&](f32x16& s, int buf, int half, int key0) {
+    float offset = 0.f;
+    if constexpr (MODE == MASKED_LINEAR) {
+      const float rel = (float)(pos - key0 - 4 * h);             // distance of the lane's first key
+      if (key0 + 31 <= pos_first || key0 >= pos_last) {
+        const bool before = key0 + 31 <= pos_first;
+        const float up = before ? tilt : -tilt;
+#pragma unroll
+        for (int y = 0; y < 16; ++y) s[y] = up * (float)(8 * (y >> 2) + (y & 3));
+        offset = (before ? -slope : slope) * rel;
+      } else {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) s[y] = -tilt * fabsf(rel - (float)(8 * (y >> 2) + (y & 3)));
+      }
+    } else {
+#pragma unroll
+      for (int y = 0; y < 16; ++y) s[y] = 0.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma32<F16>(*(const u32x4*)(lk[buf] + half * 32 * KROW + k_lane + ks * 32), qf[ks], s);
+    return offset;
+  };
+  // scores -> values whose exponent (base 2) is factor * value + offset: PLAIN and LINEAR the scores themselves; CAP 1 / (1 +
+  // exp(2 x / cap)), as cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)) (no branch, saturates by itself; off by a few 2^-24 of
+  // cap); GENERAL exponents.
+  constexpr bool DOWN = MODE == MASKED_CAP;                      // the largest exponent has the smallest value
+  const float factor = MODE == MASKED_CAP ? -2.f * cap2 : MODE == MASKED_GENERAL ? 1.f : sc;
+  auto exponents = [&](f32x16& s, int key0, float offset) {
     if constexpr (MODE == MASKED_CAP) {
 #pragma unroll
       for (int y = 0; y < 16; ++y) s[y] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap));
       return cap2;
     }
-    float f = sc;
-    if (a.cap > 0.f) {
+    if constexpr (MODE == MASKED_GENERAL) {
+      if (a.cap > 0.f) {
 #pragma unroll
-      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
-      f = 1.f;
+        for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) s[y] *= sc;
+      }
+      const float rel = (float)(pos - key0 - 4 * h);             // distance of the lane's first key
+      if (a.slopes) {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-slope, fabsf(rel - (float)(8 * (y >> 2) + (y & 3))), s[y]);
+      }
     }
-    const float rel = (float)(pos - key0 - 4 * h);          // distance of the lane's first key
-    if (key0 + 31 <= pos_first) {                                // all keys before all rows: the bias is linear in the key
-#pragma unroll
-      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(slope, (float)(8 * (y >> 2) + (y & 3)), s[y] * f);
-      return -slope * rel;
-    }
-    if (key0 >= pos_last) {                                      // all keys behind
-#pragma unroll
-      for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(slope, -(float)(8 * (y >> 2) + (y & 3)), s[y] * f);
-      return slope * rel;
-    }
-#pragma unroll
-    for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-slope, fabsf(rel - (float)(8 * (y >> 2) + (y & 3))), s[y] * f);
-    return 0.f;
+    return offset;
   };
   auto hide = [&](f32x16& s, int key0, int buf, int half) {
     constexpr float NEVER = DOWN ? INFINITY : -INFINITY;
@@ -318,7 +339,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     float top = s[0];
 #pragma unroll
     for (int y = 1; y < 16; ++y) top = DOWN ? fminf(top, s[y]) : fmaxf(top, s[y]);
-    top = MODE == MASKED_SLOPES ? top + offset : __builtin_fmaf(top, factor, offset);
+    top = __builtin_fmaf(top, factor, offset);
     if (__any(top > m + 8.f)) {
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m, top);
@@ -335,7 +356,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     const float off = offset - (m == -INFINITY ? 0.f : m);
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
-      s[y] = __builtin_amdgcn_exp2f(MODE == MASKED_SLOPES ? s[y] + off : __builtin_fmaf(s[y], factor, off));
+      s[y] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y], factor, off));
       l += s[y];
     }
   };
@@ -373,8 +394,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s])); // (arrived before the loop: a wait inside it would be for the tile loads too)
     __syncthreads();
     f32x16 s;
-    scores(s, 0, 0);
-    float offset = exponents(s, t0 * KT);
+    float offset = scores(s, 0, 0, t0 * KT);
+    offset = exponents(s, t0 * KT, offset);
     while (true) {
       const int next = buf == 2 ? 0 : buf + 1;
 #pragma unroll
@@ -385,18 +406,20 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           // states in front of an accumulator read behind such a branch, and the last product's terms were missing.)
           if (is_edge(doc0, key0)) {
             edges = true;
-            hide(s, key0, buf, half);
+            if (doc0 == OTHER) offset = -INFINITY;                // (no weight; a step that is left out would tear the pipeline)
+            else hide(s, key0, buf, half);
           }
           raise(s, offset);
           f32x16 n;
-          scores(n, half + 1 < H ? buf : next, half + 1 < H ? half + 1 : 0);   // (behind the last tile: not used)
+          const int key1 = half + 1 < H ? key0 + 32 : t1 * KT;   // (behind the last tile: not used)
+          const float offset1 = scores(n, half + 1 < H ? buf : next, half + 1 < H ? half + 1 : 0, key1);
           weights(s, offset);
           const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
 #pragma unroll
           for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
 #pragma unroll
           for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 1, x), p1, o[x]);
-          offset = exponents(n, half + 1 < H ? key0 + 32 : t1 * KT);
+          offset = exponents(n, key1, offset1);
           s = n;
         }
         if (half == 0) {
@@ -442,8 +465,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           if (key0 >= hi) break;
           const bool edge = is_edge(doc, key0);
           f32x16 s;
-          scores(s, 0, half);
-          const float offset = exponents(s, key0);
+          float offset = scores(s, 0, half, key0);
+          offset = exponents(s, key0, offset);
           if (edge) hide(s, key0, 0, half);
           raise(s, offset);
           weights(s, offset);
@@ -517,7 +540,8 @@ template <bool F16, int DP>
 void launch_masked_mode(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
   if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN><<<dim3(blocks), 512, 0, st>>>(a);
   else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP><<<dim3(blocks), 512, 0, st>>>(a);
-  else k_attn_masked<F16, DP, MASKED_SLOPES><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_LINEAR) k_attn_masked<F16, DP, MASKED_LINEAR><<<dim3(blocks), 512, 0, st>>>(a);
+  else k_attn_masked<F16, DP, MASKED_GENERAL><<<dim3(blocks), 512, 0, st>>>(a);
 }
 template <bool F16>
 int launch_masked(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {

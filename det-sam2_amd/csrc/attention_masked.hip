@@ -31,10 +31,21 @@ Plan plan_of(const ds2_attention_masked_args& a) {
   p.row_tiles = (int)cdiv64(rows, 256 / masked_value_split(a.D));
   p.heads = a.B * a.Hkv;
   p.tiles = cdiv(a.Lk, masked_tile(a.D));
-  // Fewer workgroups than CUs: the keys are split so that about two workgroups a CU result, at least 4 tiles each.
+  // Fewer workgroups than CUs: the keys are split where that is faster.  What a split saves are steps of 32 keys one after the other,
+  // 0.8 us up to 64 elements a row (1.3 us for two workgroups on a CU), 1.0 up to 96, 1.15 up to 128, 1.8 up to 256; what it costs is the
+  // join, 7 us and the parts written and read at 4 TB/s.  (32 over 8 heads, D = 128, 1024 tokens: one part 40 us, four parts 60; 4 over 1,
+  // D = 64, 4096 tokens over 28736: eight parts 184, two 332.)
   const int64_t whole = (int64_t)p.row_tiles * p.heads;
   p.parts = 1;
-  if (whole < 256) p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(p.tiles / 4, 512 / whole));
+  if (whole > 0 && whole < 256) {
+    const double part_us = (double)a.B * a.Lq * a.Hq * a.D * 8 / 4e6, step_us = a.D > 128 ? 1.8 : a.D > 96 ? 1.15 : a.D > 64 ? 1.0 : 0.8;
+    double best = 1e300;
+    for (int n = 1; n <= std::max(1, std::min(p.tiles / 2, 64)); ++n) {
+      const int64_t on_cu = cdiv64(whole * n, 256);
+      const double us = cdiv(p.tiles, n) * (masked_tile(a.D) / 32) * step_us * (a.D <= 64 && on_cu > 1 ? on_cu * 0.81 : on_cu) + (n > 1 ? 7 + n * part_us : 0);
+      if (us < best) best = us, p.parts = n;
+    }
+  }
   p.tiles_a_part = std::max(1, cdiv(p.tiles, p.parts));
   p.parts = std::max(1, cdiv(p.tiles, p.tiles_a_part));
   p.blocks = whole * p.parts;
