@@ -28,6 +28,7 @@ inline int attn_join_lanes(int D) { return D <= 32 ? 8 : D <= 64 ? 16 : D <= 128
 
 template <bool F16, bool WIDE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
+  ds2_ask_args(a);
   __shared__ __attribute__((aligned(16))) float sum[3][260];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;

@@ -406,6 +406,7 @@ constexpr int cache_residents(int D) { return D > 128 ? 2 : D > 64 ? 3 : 4; }
 
 template <int FORMAT, bool QF16, int KS, int E, int VS>
 __global__ __launch_bounds__(256, cache_residents(32 * KS)) void k_cache_attn(CacheAttnArgs a) {
+  ds2_ask_args(a);
   typedef CacheStream<FORMAT, QF16, KS, E, VS> Stream;
   constexpr bool FULL = Stream::FULL;
   constexpr int KW = 4 / VS;                               // waves of a workgroup that share its keys (or hold different rows)
@@ -434,16 +435,16 @@ __global__ __launch_bounds__(256, cache_residents(32 * KS)) void k_cache_attn(Ca
   } else {
     int sum = units_of(len0);
     for (int x = lane + 64; x < a.B; x += 64) sum += units_of(max(0, min(a.lens[x], a.C)));
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) sum += __shfl_xor(sum, s);
+#pragma unroll 1
+    for (int s = 1; s < 64 && s < a.B; s <<= 1) sum += __shfl_xor(sum, s);           // (lanes from B on hold zeros)
     const int total = __builtin_amdgcn_readfirstlane(sum) * heads, each = max(1, (total + a.shares - 1) / a.shares);
     at = share * each, end = min(total, at + each);
     if (at >= end) return;
     for (int b0 = 0;; b0 += 64) {                          // the sequence in which the share begins
       int x = (b0 == 0 ? units_of(len0) : b0 + lane < a.B ? units_of(max(0, min(a.lens[b0 + lane], a.C))) : 0) * heads;
       const int mine = x;
-#pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
+#pragma unroll 1
+      for (int s = 1; s < 64 && s < a.B; s <<= 1) {
         const int y = __shfl_up(x, s);
         x += lane >= s ? y : 0;
       }

@@ -16,6 +16,7 @@ struct WriteArgs {
 // of the head-major cache.
 template <int TYPE, int FORMAT>
 __global__ __launch_bounds__(256) void k_cache_write(WriteArgs a) {
+  ds2_ask_args(a);
   const unsigned blk = blockIdx.x, head = blk / a.blocks_per_head, part = blk - head * a.blocks_per_head;
   const int which = head >= (unsigned)a.BH;
   const int bh = head - which * a.BH, b = bh / a.H, h = bh - b * a.H;
@@ -90,6 +91,7 @@ struct ReadArgs {
 // One thread turns 16 codes (16 or 8 bytes) into 16 values.
 template <int TYPE, int FORMAT>
 __global__ __launch_bounds__(256) void k_cache_read(ReadArgs a) {
+  ds2_ask_args(a);
   const unsigned blk = blockIdx.x, bh = blk / a.blocks_per_head, part = blk - bh * a.blocks_per_head;
   const int b = bh / a.H, h = bh - b * a.H;
   const unsigned units = a.D >> 4;
