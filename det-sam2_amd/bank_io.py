@@ -17,6 +17,11 @@ Header: ``{"version": 1, "model": cfg name, "layout": "token-major", "num_frames
 conditioning frames, ``fpn2`` f32 [4096,256]: the frame's level-2 image feature, the only thing the online
 new-object path (A17, sam2_video_predictor.py:281-310) needs from a preload frame - so NO frames are stored.
 
+On request (``features="mxfp8"`` / ``"mxfp4"``) the memory features, 512 KiB of an entry and object, are stored as rows of a
+token cache of one head: ``maskmem_codes`` u8 [B,1,4096,64 or 32] and ``maskmem_scales`` u8 [B,1,4096,2] (264 or 136 KiB;
+the format is in include/detsam2_hip.h).  Such a file has ``"version": 2`` and ``"features": format`` in its header; a
+bf16 file is version 1, byte for byte as before.
+
 ``load_bank`` also reads a reference-produced pickle (through an unpickler restricted to tensors / containers) and
 converts it to the same in-memory form, so banks written by the reference stay usable.
 """
@@ -33,9 +38,12 @@ import numpy as np
 import torch
 
 MAGIC = b"DS2BANK1"
-_DT = {"bf16": (torch.bfloat16, 2), "f32": (torch.float32, 4), "f16": (torch.float16, 2)}
-_NAME = {torch.bfloat16: "bf16", torch.float32: "f32", torch.float16: "f16"}
+_DT = {"bf16": (torch.bfloat16, 2), "f32": (torch.float32, 4), "f16": (torch.float16, 2), "u8": (torch.uint8, 1)}
+_NAME = {torch.bfloat16: "bf16", torch.float32: "f32", torch.float16: "f16", torch.uint8: "u8"}
 ENTRY_TENSORS = ("maskmem_features", "pred_masks", "obj_ptr", "object_score_logits")
+PACKED_TENSORS = ("maskmem_codes", "maskmem_scales") + ENTRY_TENSORS[1:]
+FEATURE_FORMATS = ("bf16", "mxfp8", "mxfp4")
+CODE_BYTES = {"mxfp8": 64, "mxfp4": 32}          # of a row of 64 features
 
 
 def _raw(t: torch.Tensor) -> bytes:
@@ -43,13 +51,21 @@ def _raw(t: torch.Tensor) -> bytes:
     return t.view(torch.uint8).numpy().tobytes() if t.numel() else b""
 
 
-def save_bank(path, inference_state, model_name: str, fpn2_of=None) -> dict:
+def save_bank(path, inference_state, model_name: str, fpn2_of=None, features: str = "bf16", pack=None) -> dict:
     """Write the conditioning / non-conditioning entries and the object table of ``inference_state``.
-    ``fpn2_of(frame_idx) -> tensor [4096,256] | None`` supplies the level-2 feature of a conditioning frame."""
+    ``fpn2_of(frame_idx) -> tensor [4096,256] | None`` supplies the level-2 feature of a conditioning frame.
+    ``features``: how memory features are stored; ``pack(features, format) -> (codes, scales)`` (``HipOps.pack_features``)
+    is needed for the quantised formats."""
+    if features not in FEATURE_FORMATS:
+        raise ValueError(f"bank features must be one of {FEATURE_FORMATS}, got {features!r}")
+    if features != "bf16" and pack is None:
+        raise ValueError(f"bank features {features!r} need a packing function")
     st = inference_state
     hdr = {"version": 1, "model": model_name, "layout": "token-major", "num_frames": int(st["num_frames"]),
            "video_height": int(st["video_height"]), "video_width": int(st["video_width"]),
            "obj_ids": [int(o) for o in st["obj_ids"]], "entries": []}
+    if features != "bf16":
+        hdr.update(version=2, features=features)
     blobs, off = [], 0
 
     def add(t):
@@ -65,9 +81,17 @@ def save_bank(path, inference_state, model_name: str, fpn2_of=None) -> dict:
 
     for kind, key in (("cond", "cond_frame_outputs"), ("non_cond", "non_cond_frame_outputs")):
         for t, out in st["output_dict"][key].items():
-            if out.get("maskmem_features") is None:
+            if out.get("maskmem_codes") is not None:         # read from a quantised file and not unpacked since
+                if features != out["maskmem_format"]:
+                    raise ValueError(f"bank entry of frame {t} holds {out['maskmem_format']} features: unpack them (init_preloading_state) "
+                                     f"before they are saved as {features}")
+            elif out.get("maskmem_features") is None:
                 continue
-            rec = {"frame": int(t), "kind": kind, "tensors": {k: add(out[k]) for k in ENTRY_TENSORS}}
+            elif features != "bf16":
+                codes, scales = pack(out["maskmem_features"], features)
+                out = dict(out, maskmem_codes=codes, maskmem_scales=scales)
+            names = ENTRY_TENSORS if features == "bf16" else PACKED_TENSORS
+            rec = {"frame": int(t), "kind": kind, "tensors": {k: add(out[k]) for k in names}}
             if kind == "cond" and fpn2_of is not None:
                 f2 = fpn2_of(int(t))
                 if f2 is not None:
@@ -111,7 +135,8 @@ def _read_ds2bank(f) -> dict:
     if n > (64 << 20):
         raise ValueError("DS2BANK header too large")
     hdr = json.loads(f.read(n).decode())
-    if hdr.get("version") != 1 or hdr.get("layout") != "token-major":
+    packed = hdr.get("features") if hdr.get("version") == 2 else None
+    if hdr.get("version") not in (1, 2) or hdr.get("layout") != "token-major" or (hdr["version"] == 2 and packed not in CODE_BYTES):
         raise ValueError(f"unsupported DS2BANK version/layout: {hdr.get('version')}/{hdr.get('layout')}")
     f.seek((16 + n + 63) // 64 * 64)
     payload = f.read()
@@ -128,10 +153,17 @@ def _read_ds2bank(f) -> dict:
 
     for e in hdr["entries"]:
         key = "cond_frame_outputs" if e["kind"] == "cond" else "non_cond_frame_outputs"
-        out = {k: get(e["tensors"][k]) for k in ENTRY_TENSORS}
+        out = {k: get(e["tensors"][k]) for k in (PACKED_TENSORS if packed else ENTRY_TENSORS)}
         out["maskmem_pos_enc"] = None
         B = out["obj_ptr"].shape[0]
-        if tuple(out["maskmem_features"].shape) != (B, 4096, 64) or tuple(out["pred_masks"].shape) != (B, 1, 256, 256):
+        if packed:                                   # unpacked where the state goes: init_preloading_state
+            out["maskmem_features"], out["maskmem_format"] = None, packed
+            good = all(out[k].dtype == torch.uint8 for k in PACKED_TENSORS[:2]) \
+                and tuple(out["maskmem_codes"].shape) == (B, 1, 4096, CODE_BYTES[packed]) \
+                and tuple(out["maskmem_scales"].shape) == (B, 1, 4096, 2)
+        else:
+            good = tuple(out["maskmem_features"].shape) == (B, 4096, 64)
+        if not good or tuple(out["pred_masks"].shape) != (B, 1, 256, 256):
             raise ValueError(f"DS2BANK entry of frame {e['frame']} has unexpected shapes")
         st["output_dict"][key][int(e["frame"])] = out
         st["frames_already_tracked"][int(e["frame"])] = {"reverse": True}    # as in a reference pickle (:1013-1016)

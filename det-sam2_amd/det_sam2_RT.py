@@ -87,7 +87,10 @@ class VideoProcessor:
                  detect_model_weights=None, detect_confidence=0.85, skip_classes={11, 14, 15, 19}, vis_frame_stride=-1,
                  visualize_prompt=False, frame_buffer_size=30, detect_interval=30, max_frame_num_to_track=60,
                  max_inference_state_frames=60, load_inference_state_path=None, save_inference_state_path=None,
-                 detector=None, device="cuda", predictor=None):
+                 detector=None, device="cuda", predictor=None, bank_format="bf16"):
+        if bank_format not in bank_io.FEATURE_FORMATS:
+            raise ValueError(f"bank_format must be one of {bank_io.FEATURE_FORMATS}, got {bank_format!r}")
+        self.bank_format = bank_format
         self.output_dir = output_dir
         self.sam2_checkpoint, self.model_cfg = sam2_checkpoint, model_cfg
         self.detect_model_weights, self.detect_confidence = detect_model_weights, detect_confidence
@@ -223,7 +226,8 @@ class VideoProcessor:
     def save_inference_state(self, save_path):
         """det_sam2_RT.py:489-497.  The reference pickles the whole state (frames, devices, views); here the bank goes
         into a versioned tensor file (bank_io.DS2BANK: cond / non-cond entries + object table + the level-2 feature of
-        every conditioning frame; no pickle, no frames)."""
+        every conditioning frame; no pickle, no frames).  ``bank_format``: memory features as they are (bf16), or as 8- or
+        4-bit rows of a token cache (mxfp8: 264 KiB of a frame and object instead of 512, mxfp4: 136)."""
         os.makedirs(os.path.dirname(save_path) or ".", exist_ok=True)
         st = self.inference_state
 
@@ -234,7 +238,10 @@ class VideoProcessor:
                 return self.predictor._get_image_feature(st, t)[2]
             return None
 
-        bank_io.save_bank(save_path, st, self.predictor.cfg.name, fpn2_of)
+        if self.bank_format == "bf16":
+            bank_io.save_bank(save_path, st, self.predictor.cfg.name, fpn2_of)
+        else:
+            bank_io.save_bank(save_path, st, self.predictor.cfg.name, fpn2_of, self.bank_format, self.predictor.hip.pack_features)
 
     def load_inference_state(self, load_path):
         """det_sam2_RT.py:499-503: DS2BANK files, and inference-state pickles written by the reference (read through a

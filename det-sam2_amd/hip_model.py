@@ -78,6 +78,50 @@ class HipOps:
         _capi.check(self.lib.ds2_profile_tags(buf, len(buf)), "ds2_profile_tags")
         return [t for t in buf.value.decode().split("\n") if t]
 
+    # ------------------------------------------------------------------ token cache
+    def cache_alloc(self, B, H, C, D, format, pair=True):
+        """Empty codes uint8 [B,H,C,D or D/2] and scales uint8 [B,H,C,D/32] of a quantised cache ("mxfp8", "mxfp4") of C tokens
+        -> (k_codes, k_scales, v_codes, v_scales), or the first two for ``pair=False``."""
+        if format not in ("mxfp8", "mxfp4"):
+            raise ValueError(f"cache format must be 'mxfp8' or 'mxfp4', got {format!r}")
+        if D % 32:
+            raise ValueError(f"rows of a quantised cache have a multiple of 32 values, got {D}")
+        return tuple(self._empty(B, H, C, w, dtype=torch.uint8) for w in (D if format == "mxfp8" else D // 2, D // 32) * (2 if pair else 1))
+
+    def cache_write(self, k, pos, k_codes, k_scales, format, v=None, v_codes=None, v_scales=None, count=None):
+        """Rows k (and v) [B,T,H,D] (bf16, fp16 or fp32) to rows pos[b] + t of the cache, t < count[b] (None: all T); rows that
+        fall outside the cache are dropped, all others stay as they are (ds2_op_cache_write)."""
+        self.ops.cache_write(k, v, pos, count, k_codes, k_scales, v_codes, v_scales, format)
+
+    def cache_read(self, codes, scales, format, lens=None, dtype=torch.bfloat16):
+        """The values [B,H,C,D] that a quantised cache stands for; rows from lens[b] on are zero (ds2_op_cache_read)."""
+        return self.ops.cache_read(codes, scales, lens, format, dtype)
+
+    def cache_attention(self, q, k, v, lens, *, scale, format="plain", k_scales=None, v_scales=None, prefix_k=None, prefix_v=None,
+                        prefix_k_scales=None, prefix_v_scales=None, cap=0.0, slopes=None):
+        """Attention of the last T of lens[b] tokens, q [B,T,Hq,D], over a cache k, v [B,Hkv,C,...] in q's type or quantised, behind
+        an optional prefix [Hkv,P,...] that all sequences share -> [B,T,Hq,D] (ds2_op_cache_attention)."""
+        return self.ops.cache_attention(q, k, v, k_scales, v_scales, lens, prefix_k, prefix_v, prefix_k_scales, prefix_v_scales, format,
+                                        scale, cap, slopes)
+
+    def attention_masked(self, q, k, v, *, scale, causal=False, cap=0.0, slopes=None, lens=None, q_start=None, prefix=None, q_doc=None,
+                         k_doc=None):
+        """Attention of whole prompts, q [B,Lq,Hq,D] over k, v [B,Lk,Hkv,D], with causal, prefix, length and document masks, capped
+        scores and distance bias -> [B,Lq,Hq,D] (ds2_op_attention_masked)."""
+        return self.ops.attention_masked(q, k, v, scale, causal, cap, slopes, lens, q_start, prefix, q_doc, k_doc)
+
+    def pack_features(self, features, format):
+        """Memory features [B,N,64] -> (codes, scales) of a cache of one head, on the device."""
+        f = features.to(self.device).contiguous()
+        B, N, D = f.shape
+        codes, scales = self.cache_alloc(B, 1, N, D, format, pair=False)
+        self.cache_write(f.view(B, N, 1, D), torch.zeros(B, dtype=torch.int32, device=self.device), codes, scales, format)
+        return codes, scales
+
+    def unpack_features(self, codes, scales, format):
+        """(codes, scales) of ``pack_features`` -> bf16 memory features [B,N,64] on the device."""
+        return self.cache_read(codes.to(self.device), scales.to(self.device), format).squeeze(1)
+
     # ------------------------------------------------------------------ primitives (tests)
     def op_gemm(self, A, W, bias=None, act=0, gamma=None, R=None, r_mod=0):
         M, K = A.shape

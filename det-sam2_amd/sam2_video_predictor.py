@@ -151,6 +151,8 @@ class SAM2VideoPredictor:
         for key in ("cond_frame_outputs", "non_cond_frame_outputs"):
             for t, out in st["output_dict"][key].items():
                 f = out.get("maskmem_features")
+                if out.get("maskmem_codes") is not None:   # a bank file with quantised features
+                    f = self.hip.unpack_features(out.pop("maskmem_codes"), out.pop("maskmem_scales"), out.pop("maskmem_format"))
                 if f is not None and f.dim() == 4:       # a reference-layout state handed over directly (not via load_bank)
                     f = f.flatten(2).transpose(1, 2).contiguous().to(torch.bfloat16)
                 if f is not None and tuple(f.shape[1:]) != (4096, 64):
