@@ -21,17 +21,20 @@ struct AttnJoinArgs {
 };
 
 // Latency is what this kernel is made of (2 to 5 us for a few MB), so little of it is one after the other: D / 4 lanes (rounded up
-// to a power of two) are a reader of parts, a wave holds 64 / that many readers, WIDE four times as many (a row for the workgroup's
-// four waves); every reader asks for statistics and rows of eight parts at once and weighs them against a running maximum.  A row of
-// up to eight parts a reader waits for memory twice: for where its parts are, and for the parts.
+// to a power of two) are a reader of parts, and every reader asks for statistics and rows of eight parts at once and weighs them against
+// a running maximum.  A row of up to eight parts is one reader's (NARROW), one of more the readers' of a wave (ROW) or of four (WIDE),
+// eight parts each as far as that reaches: it waits for memory twice, for where its parts are and for the parts.
+enum { JOIN_NARROW = 0, JOIN_ROW = 1, JOIN_WIDE = 2 };
 inline int attn_join_lanes(int D) { return D <= 32 ? 8 : D <= 64 ? 16 : D <= 128 ? 32 : 64; }
 
-template <bool F16, bool WIDE>
+template <bool F16, int MODE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
   ds2_ask_args(a);
+  constexpr bool WIDE = MODE == JOIN_WIDE;
   __shared__ __attribute__((aligned(16))) float sum[3][260];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  const int each = a.lanes, readers = 64 / each, reader = lane / each;
+  const int64_t row = WIDE ? (int64_t)blockIdx.x : MODE == JOIN_ROW ? (int64_t)blockIdx.x * 4 + wave : ((int64_t)blockIdx.x * 4 + wave) * readers + reader;
   if (row >= a.rows) return;
   int parts = a.parts;
   int64_t seg = 0;                                           // index of part p, p >= a.parts, is seg + p own_rows
@@ -48,8 +51,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
     }
     none = len - a.T + t < 0;
   }
-  const int each = a.lanes, readers = 64 / each;
-  const int first = (WIDE ? wave * readers : 0) + lane / each, step = (WIDE ? 4 : 1) * readers;
+  const int first = MODE == JOIN_NARROW ? 0 : (WIDE ? wave * readers : 0) + reader, step = MODE == JOIN_NARROW ? 1 : (WIDE ? 4 : 1) * readers;
   const int d = (lane & (each - 1)) * 4;
   const bool live = d < a.D;
   f32x4 o = {0, 0, 0, 0};
@@ -68,12 +70,14 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
     f32x4 x[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int p = min(p0 + u * step, parts - 1);
-      const bool own = p >= a.parts;
-      const int64_t at = own ? seg + (int64_t)p * a.own_rows : p * a.rows + row;
-      ml[u] = (own ? a.seg_ml : a.ml)[at];
-      x[u] = live ? *(const f32x4*)((own ? a.seg_o : a.o) + at * a.D + d) : f32x4{0, 0, 0, 0};
-      if (p0 + u * step >= parts) ml[u] = f32x2_t{-INFINITY, 0.f};
+      const int p = p0 + u * step;
+      ml[u] = f32x2_t{-INFINITY, 0.f}, x[u] = f32x4{0, 0, 0, 0};
+      if (p < parts) {
+        const bool own = p >= a.parts;
+        const int64_t at = own ? seg + (int64_t)p * a.own_rows : p * a.rows + row;
+        ml[u] = (own ? a.seg_ml : a.ml)[at];
+        if (live) x[u] = *(const f32x4*)((own ? a.seg_o : a.o) + at * a.D + d);
+      }
     }
     float mn = m;
 #pragma unroll
@@ -83,7 +87,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
     for (int u = 0; u < 8; ++u)
       if (!(ml[u][0] == -INFINITY && ml[u][1] == 0.f)) add(ml[u][0], ml[u][1], x[u]);    // (a part that saw nothing may not have written its row)
   }
-  for (int s = each; s < 64; s <<= 1) {                      // the wave's readers
+  for (int s = each; MODE != JOIN_NARROW && s < 64; s <<= 1) {       // the wave's readers
     const float mo = __shfl_xor(m, s), lo = __shfl_xor(l, s);
     const f32x4 oo = {__shfl_xor(o[0], s), __shfl_xor(o[1], s), __shfl_xor(o[2], s), __shfl_xor(o[3], s)};
     raise(fmaxf(m, mo));
@@ -102,20 +106,25 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnJoinArgs a) {
       add(sum[w][257], sum[w][256], *(const f32x4*)&sum[w][d]);
     }
   }
-  if (!live || lane >= each) return;
+  if (!live || (MODE != JOIN_NARROW && lane >= each)) return;
   none |= m == -INFINITY && l == 0.f;                        // nothing seen: zeros
   const float f = 1.f / l;
   *(u32x2*)(a.out + (row * a.D + d) * 2) =
       none ? u32x2{0, 0} : u32x2{ds2_pack16<F16>(o[0] * f, o[1] * f), ds2_pack16<F16>(o[2] * f, o[3] * f)};
 }
 
-// usual_parts: of a row, as far as the host knows; over eight of them a reader, four waves share a row
+// usual_parts: of a row, as far as the host knows
+template <bool F16>
+void launch_attn_join_of(const AttnJoinArgs& a, int64_t usual_parts, hipStream_t st) {
+  const int readers = 64 / a.lanes;
+  if (usual_parts <= 8) k_attn_join<F16, JOIN_NARROW><<<dim3((unsigned)cdiv64(a.rows, 4 * readers)), 256, 0, st>>>(a);
+  else if (usual_parts <= 8 * readers) k_attn_join<F16, JOIN_ROW><<<dim3((unsigned)cdiv64(a.rows, 4)), 256, 0, st>>>(a);
+  else k_attn_join<F16, JOIN_WIDE><<<dim3((unsigned)a.rows), 256, 0, st>>>(a);
+}
 inline int launch_attn_join(AttnJoinArgs a, bool f16, int64_t usual_parts, hipStream_t st) {
   a.lanes = attn_join_lanes(a.D);
-  const bool wide = usual_parts > 8 * (64 / a.lanes);
-  const dim3 grid((unsigned)(wide ? a.rows : cdiv64(a.rows, 4)));
-  if (f16) wide ? k_attn_join<true, true><<<grid, 256, 0, st>>>(a) : k_attn_join<true, false><<<grid, 256, 0, st>>>(a);
-  else wide ? k_attn_join<false, true><<<grid, 256, 0, st>>>(a) : k_attn_join<false, false><<<grid, 256, 0, st>>>(a);
+  if (f16) launch_attn_join_of<true>(a, usual_parts, st);
+  else launch_attn_join_of<false>(a, usual_parts, st);
   DS2_CHECK_LAUNCH();
   return DS2_OK;
 }
