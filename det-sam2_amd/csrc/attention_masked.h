@@ -20,7 +20,15 @@
 //    not visited, steps below every row's limit are not masked.  Documents: a small kernel notes the smallest and largest document of
 //    each key tile; a wave-wide vote over 64 tiles at a time finds the tiles that can hold a visible pair.
 //  * The running maximum is raised only by more than 2^8: the weights stay below 2^8 and the rescaling of O is rare.
+//  * Where 256 rows a workgroup would leave CUs idle or unevenly loaded, the eight waves hold 128 rows twice (KG = 2): each takes every
+//    other step of the tiles, and the two halves are joined through LDS at the end (attention_masked.hip has the rule).
 //  * Weights are rounded to the operands' 16-bit type before the value product: one rounding of half a step, like the output's own.
+//
+// Measured (16-bit operands in, TFLOP/s over the visible pairs): D = 128, 32 over 8 heads, 8192 tokens: full 967, causal 945, capped
+// 830, distance bias 895; a plain library product of 16-bit matrices makes 1096 on the same card.  D = 64, 16 heads, 8190 tokens: 730,
+// causal 637; D = 256, 8 over 2 heads, 4096 tokens: 595.  At D = 128 the matrix pipes are busy 43 % of the cycles, the vector pipe
+// 39 %, LDS 27 %; other orders of a step, priorities, and halves of the workgroup in opposite phases all took the same time or more.
+// At D = 64 the exponentials (a quarter of the vector rate) carry more weight: vector pipe 68 %, matrix pipes 41 %.
 #pragma once
 #include "token_cache.h"
 
@@ -32,7 +40,9 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
 // Over 128 output elements a row, two waves take half of them each and both compute the scores: 128 accumulators and 64 query
 // registers a wave leave no room for the pipeline.
 constexpr int masked_value_split(int D) { return D > 128 ? 2 : 1; }
-constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }     // keys of a tile
+// rows of a workgroup
+constexpr int masked_rows(int D, int key_groups) { return 256 / masked_value_split(D) / key_groups; }
+constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }   // keys of a tile
 constexpr float LOG2E = 1.44269504088896340736f;
 // How scores become exponents.  LINEAR: distance bias without a cap, by what the products start from; GENERAL: cap and bias, or a scale
 // that the others do not take.  (D = 64, 16 heads, 8190 tokens with a bias: GENERAL 659 TFLOP/s, LINEAR 727, PLAIN without it 726.)
@@ -51,6 +61,7 @@ struct MaskedArgs {
   const int2* tile_docs;                    // [B][tiles]: smallest (-1: a key of none among them) and largest document of a tile
   int B, Lq, Lk, Hq, Hkv, G, D, causal;
   float scale, cap;
+  int key_groups;                           // waves that share rows and take every other step (masked_rows)
   int row_tiles, heads, parts, tiles, tiles_a_part, fold;
   float* part_o;                            // null: one part
   f32x2_t* part_ml;
@@ -80,19 +91,24 @@ __device__ __forceinline__ unsigned not_finite(unsigned w) {
 
 // The register limit keeps accumulators out of the AGPRs.  With them, and a divergent branch in the tile loop, hipcc placed copies into
 // AGPRs in front of the restored lane mask; the loop below has wave-uniform branches only.
-template <bool F16, int DP, int MODE>
+template <bool F16, int DP, int MODE, int KG>
 __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs a) {
   ds2_ask_args(a);
   constexpr int NW = 8;                                          // waves (those without rows of their own stage keys for the others)
-  constexpr int KT = masked_tile(DP), H = KT / 32;               // steps of a tile
-  constexpr int VS = masked_value_split(DP), RW = NW / VS;       // waves that share rows (each takes 1 / VS of the output), waves of other rows
+  constexpr int KT = masked_tile(DP), H = KT / 32, ST = H / KG;  // steps of a tile, a wave's
+  constexpr int VS = masked_value_split(DP), RW = NW / VS / KG;  // waves that share rows (each takes 1 / VS of the output or 1 / KG of the keys), waves of other rows
+  static_assert(KG == 1 || (VS == 1 && H == 2));
   constexpr bool BIAS = MODE >= MASKED_LINEAR;
   constexpr int KS = DP / 16, DB = DP / 32 / VS;                 // contraction steps of a score, a wave's blocks of 32 output elements
   constexpr int KROW = DP * 2 + 16, VROW = DP == 32 ? 64 : DP == 64 ? 192 : DP == 96 ? 192 : DP == 128 ? 320 : 576;
   constexpr int CH = DP / 8;                                     // 16-byte pieces of a row
   constexpr int NT = NW * 64, PER = (KT * CH + NT - 1) / NT;     // pieces a thread stages of a K (and of a V) tile
-  __shared__ __attribute__((aligned(16))) unsigned char lk[3][KT * KROW + 16];     // (+ 16: where threads without a piece write)
-  __shared__ __attribute__((aligned(16))) unsigned char lv[3][KT * VROW + 16];
+  constexpr int KBUF = KT * KROW + 16, VBUF = KT * VROW + 16;    // (+ 16: where threads without a piece write)
+  typedef float Joined[DB * 16 + 2][64];                         // what a wave of the second key group hands over, by lane
+  static_assert(KG == 1 || RW * sizeof(Joined) <= 3 * (KBUF + VBUF));
+  __shared__ __attribute__((aligned(16))) unsigned char lds[3 * (KBUF + VBUF)];
+  unsigned char(*const lk)[KBUF] = (unsigned char(*)[KBUF])lds;
+  unsigned char(*const lv)[VBUF] = (unsigned char(*)[VBUF])(lds + 3 * KBUF);
   __shared__ int ldoc[3][64];
   __shared__ int wg_lim[NW][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -119,7 +135,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   const int b = head / a.Hkv, kvh = head - b * a.Hkv;
   const int rows = a.G * a.Lq;
   const int row0 = rt * RW * 32 + wave % RW * 32;                // the wave's rows of this key head
-  const int d0 = wave / RW * DB * 32;                            // and its first output element
+  const int d0 = VS > 1 ? wave / RW * DB * 32 : 0;               // its first output element
+  const int kg = KG > 1 ? wave / RW : 0;                         // its first step of a tile
   const int r = min(row0 + c, rows - 1);                         // rows behind the last repeat it and are not written
   const int i = r / a.G, hq = kvh * a.G + (r - i * a.G);
   const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
@@ -395,13 +412,13 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s])); // (arrived before the loop: a wait inside it would be for the tile loads too)
     __syncthreads();
     f32x16 s;
-    float offset = scores(s, 0, 0, t0 * KT);
-    offset = exponents(s, t0 * KT, offset);
+    float offset = scores(s, 0, kg, t0 * KT + kg * 32);
+    offset = exponents(s, t0 * KT + kg * 32, offset);
     while (true) {
       const int next = buf == 2 ? 0 : buf + 1;
 #pragma unroll
-      for (int half = 0; half < H; ++half) {
-        const int key0 = t0 * KT + half * 32;
+      for (int st = 0; st < ST; ++st) {
+        const int half = kg + st, key0 = t0 * KT + half * 32;
         if (key0 < hi) {                                         // (keys ascend: a wave that is done stays done)
           // (The edge is decided before any product: no branch between score products and their first use - hipcc left out the wait
           // states in front of an accumulator read behind such a branch, and the last product's terms were missing.)
@@ -412,8 +429,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           }
           raise(s, offset);
           f32x16 n;
-          const int key1 = half + 1 < H ? key0 + 32 : t1 * KT;   // (behind the last tile: not used)
-          const float offset1 = scores(n, half + 1 < H ? buf : next, half + 1 < H ? half + 1 : 0, key1);
+          const int key1 = st + 1 < ST ? key0 + 32 : t1 * KT + kg * 32;          // (behind the last tile: not used)
+          const float offset1 = scores(n, st + 1 < ST ? buf : next, st + 1 < ST ? half + 1 : kg, key1);
           weights(s, offset);
           const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
 #pragma unroll
@@ -423,7 +440,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           offset = exponents(n, key1, offset1);
           s = n;
         }
-        if (half == 0) {
+        if (st == 0) {
           if (t2 < t_end) stage(tile, next == 2 ? 0 : next + 1);       // (that buffer was last read before this tile's barrier)
           t3 = next_tile(t2 + 1), doc3 = tile_doc(t3);
           if (t3 < t_end) fetch(tile, t3);
@@ -461,7 +478,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
         stage(tile, 0);
         __syncthreads();
 #pragma unroll 1
-        for (int half = 0; half < H; ++half) {
+        for (int half = kg; half < kg + ST; ++half) {
           const int key0 = t * KT + half * 32;
           if (key0 >= hi) break;
           const bool edge = is_edge(doc, key0);
@@ -506,6 +523,26 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   }
 
   l += __shfl_xor(l, 32);
+  if constexpr (KG > 1) {                                        // join the key groups: the same rows in the same lanes
+    Joined& other = ((Joined*)lds)[wave % RW];
+    __syncthreads();                                             // (the waves are through with their keys)
+    if (kg) {
+#pragma unroll
+      for (int x = 0; x < DB; ++x)
+#pragma unroll
+        for (int y = 0; y < 16; ++y) other[x * 16 + y][lane] = o[x][y];
+      other[DB * 16][lane] = m, other[DB * 16 + 1][lane] = l;
+    }
+    __syncthreads();
+    if (kg) return;
+    const float mo = other[DB * 16][lane], mn = fmaxf(m, mo);
+    const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn), fo = mo == mn ? 1.f : __builtin_amdgcn_exp2f(mo - mn);
+    l = l * f + fo * other[DB * 16 + 1][lane], m = mn;
+#pragma unroll
+    for (int x = 0; x < DB; ++x)
+#pragma unroll
+      for (int y = 0; y < 16; ++y) o[x][y] = o[x][y] * f + fo * other[x * 16 + y][lane];
+  }
   if (row0 + c >= rows) return;
   int group = a.G;
   asm volatile("" : "+s"(group));                                // (position and head again: not kept in registers through the loop)
@@ -537,20 +574,25 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   }
 }
 
-template <bool F16, int DP>
+template <bool F16, int DP, int KG>
 void launch_masked_mode(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
-  if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN><<<dim3(blocks), 512, 0, st>>>(a);
-  else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP><<<dim3(blocks), 512, 0, st>>>(a);
-  else if (mode == MASKED_LINEAR) k_attn_masked<F16, DP, MASKED_LINEAR><<<dim3(blocks), 512, 0, st>>>(a);
-  else k_attn_masked<F16, DP, MASKED_GENERAL><<<dim3(blocks), 512, 0, st>>>(a);
+  if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN, KG><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP, KG><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_LINEAR) k_attn_masked<F16, DP, MASKED_LINEAR, KG><<<dim3(blocks), 512, 0, st>>>(a);
+  else k_attn_masked<F16, DP, MASKED_GENERAL, KG><<<dim3(blocks), 512, 0, st>>>(a);
+}
+template <bool F16, int DP>
+void launch_masked_groups(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
+  if (a.key_groups == 2) launch_masked_mode<F16, DP, 2>(a, mode, blocks, st);
+  else launch_masked_mode<F16, DP, 1>(a, mode, blocks, st);
 }
 template <bool F16>
 int launch_masked(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
-  if (a.D <= 32) launch_masked_mode<F16, 32>(a, mode, blocks, st);
-  else if (a.D <= 64) launch_masked_mode<F16, 64>(a, mode, blocks, st);
-  else if (a.D <= 96) launch_masked_mode<F16, 96>(a, mode, blocks, st);
-  else if (a.D <= 128) launch_masked_mode<F16, 128>(a, mode, blocks, st);
-  else launch_masked_mode<F16, 256>(a, mode, blocks, st);
+  if (a.D <= 32) launch_masked_groups<F16, 32>(a, mode, blocks, st);
+  else if (a.D <= 64) launch_masked_groups<F16, 64>(a, mode, blocks, st);
+  else if (a.D <= 96) launch_masked_groups<F16, 96>(a, mode, blocks, st);
+  else if (a.D <= 128) launch_masked_groups<F16, 128>(a, mode, blocks, st);
+  else launch_masked_mode<F16, 256, 1>(a, mode, blocks, st);
   DS2_CHECK_LAUNCH();
   return DS2_OK;
 }

@@ -21,31 +21,38 @@ __global__ __launch_bounds__(64) void k_tile_docs(const int32_t* doc, int Lk, in
 }
 
 struct Plan {
-  int row_tiles, heads, parts, tiles, tiles_a_part;
+  int key_groups, row_tiles, heads, parts, tiles, tiles_a_part;
   int64_t blocks, doc_bytes, part_bytes;
 };
 
 Plan plan_of(const ds2_attention_masked_args& a) {
   Plan p{};
   const int64_t rows = (int64_t)(a.Hq / a.Hkv) * a.Lq;
-  p.row_tiles = (int)cdiv64(rows, 256 / masked_value_split(a.D));
   p.heads = a.B * a.Hkv;
   p.tiles = cdiv(a.Lk, masked_tile(a.D));
-  // Fewer workgroups than CUs: the keys are split where that is faster.  What a split saves are steps of 32 keys one after the other,
-  // 0.8 us up to 64 elements a row (1.3 us for two workgroups on a CU), 1.0 up to 96, 1.15 up to 128, 1.8 up to 256; what it costs is the
-  // join, 7 us and the parts written and read at 4 TB/s.  (32 over 8 heads, D = 128, 1024 tokens: one part 40 us, four parts 60; 4 over 1,
-  // D = 64, 4096 tokens over 28736: eight parts 184, two 332.)
-  const int64_t whole = (int64_t)p.row_tiles * p.heads;
-  p.parts = 1;
-  if (whole > 0 && whole < 256) {
-    const double part_us = (double)a.B * a.Lq * a.Hq * a.D * 8 / 4e6, step_us = a.D > 128 ? 1.8 : a.D > 96 ? 1.15 : a.D > 64 ? 1.0 : 0.8;
-    double best = 1e300;
-    for (int n = 1; n <= std::max(1, std::min(p.tiles / 2, 64)); ++n) {
-      const int64_t on_cu = cdiv64(whole * n, 256);
-      const double us = cdiv(p.tiles, n) * (masked_tile(a.D) / 32) * step_us * (a.D <= 64 && on_cu > 1 ? on_cu * 0.81 : on_cu) + (n > 1 ? 7 + n * part_us : 0);
-      if (us < best) best = us, p.parts = n;
+  // How many rows a workgroup takes (the waves of half as many split its keys) and whether the keys are split over workgroups:
+  // whatever takes least time by this model.  A step of 32 keys takes a workgroup 0.8 us up to 64 elements a row (two on a CU 1.3), 1.0 up
+  // to 96, 1.15 up to 128, 1.8 up to 256, and a quarter more with its keys split over waves (every step has a barrier); the call takes as
+  // long as the longest workgroup or the work of a CU; parts cost a join, 7 us and what they write and read at 4 TB/s.  Measured, rows
+  // whole / keys split over waves: 32 over 8 heads, D = 128, causal 1024 tokens 39 / 30 us, 2048 tokens 75 / 61, four times 2048
+  // of 16 over 8 heads 98 / 123; D = 96, twice 2500 tokens of 8 over 4 heads 71 / 51.  Parts: 4 over 1 heads, D = 64, 4096 tokens over
+  // 28736 in eight parts 175 us, two 332; the 1024 tokens above in one part 39, four 60.
+  const double part_us = (double)a.B * a.Lq * a.Hq * a.D * 8 / 4e6, step_us = a.D > 128 ? 1.8 : a.D > 96 ? 1.15 : a.D > 64 ? 1.0 : 0.8;
+  const double seen = a.causal && a.Lk ? 1 - 0.5 * std::min(1.0, (double)a.Lq / a.Lk) : 1;      // of all pairs
+  double best = 1e300;
+  p.parts = p.key_groups = 1;
+  for (int kg = 1; kg <= (a.D <= 128 ? 2 : 1); ++kg) {
+    const int64_t whole = cdiv64(rows, masked_rows(a.D, kg)) * p.heads;
+    for (int n = 1; n <= (whole < 256 ? std::max(1, std::min(p.tiles / 2, 64)) : 1); ++n) {
+      const double longest = (double)cdiv(p.tiles, n) * (masked_tile(a.D) / 32) / kg;
+      const double on_cu = seen < 1 ? whole * n / 256.0 : (double)cdiv64(whole * n, 256);
+      const double steps = std::max(longest, longest * seen * on_cu * (a.D <= 64 && on_cu > 1 ? 0.81 : 1));
+      const double us = steps * step_us * (kg > 1 ? 1.25 : 1) + (n > 1 ? 7 + n * part_us : 0);
+      if (us < best) best = us, p.parts = n, p.key_groups = kg;
     }
   }
+  p.row_tiles = (int)cdiv64(rows, masked_rows(a.D, p.key_groups));
+  const int64_t whole = (int64_t)p.row_tiles * p.heads;
   p.tiles_a_part = std::max(1, cdiv(p.tiles, p.parts));
   p.parts = std::max(1, cdiv(p.tiles, p.tiles_a_part));
   p.blocks = whole * p.parts;
@@ -104,7 +111,7 @@ extern "C" int ds2_op_attention_masked(const ds2_attention_masked_args* args, vo
   a.slopes = x.slopes, a.lens = x.lens, a.q_start = x.q_start, a.prefix = x.prefix, a.q_doc = x.q_doc, a.k_doc = x.k_doc;
   a.B = x.B, a.Lq = x.Lq, a.Lk = x.Lk, a.Hq = x.Hq, a.Hkv = x.Hkv, a.G = x.Hq / x.Hkv, a.D = x.D, a.causal = x.causal;
   a.scale = x.scale, a.cap = x.cap;
-  a.row_tiles = p.row_tiles, a.heads = p.heads, a.parts = p.parts, a.tiles = p.tiles, a.tiles_a_part = p.tiles_a_part;
+  a.key_groups = p.key_groups, a.row_tiles = p.row_tiles, a.heads = p.heads, a.parts = p.parts, a.tiles = p.tiles, a.tiles_a_part = p.tiles_a_part;
   a.fold = x.causal && x.D <= 64 && p.blocks <= 512;
   hipStream_t st = (hipStream_t)stream;
   if (x.q_doc && p.tiles) {

@@ -37,7 +37,7 @@ Split split_of(const ds2_cache_attention_args& a) {
     // 256 rows (16-bit caches whose rows follow each other at one stride).
     s.tiled = a.format == DS2_CACHE_PLAIN && all_rows >= 64 && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
     if (s.tiled) {
-      s.pre_row_tiles = (int)cdiv64(all_rows, 256 / masked_value_split(a.D));
+      s.pre_row_tiles = (int)cdiv64(all_rows, masked_rows(a.D, 1));
       const int tiles = cdiv(a.prefix_len, masked_tile(a.D));
       const int64_t whole = (int64_t)a.Hkv * s.pre_row_tiles;
       s.pre_tiles = (int)std::max<int64_t>(a.D <= 64 ? 8 : 4, cdiv64(tiles * whole, 256));
@@ -163,7 +163,7 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
     m.slopes = a.slopes, m.row_lens = x.lens, m.row_T = x.T, m.row_C = x.capacity;
     m.B = 1, m.Lq = x.B * x.T, m.Lk = x.prefix_len, m.Hq = x.Hq, m.Hkv = x.Hkv, m.G = a.G, m.D = x.D;
     m.scale = x.scale, m.cap = x.cap;
-    m.row_tiles = s.pre_row_tiles, m.heads = x.Hkv, m.parts = s.pre_parts, m.tiles_a_part = s.pre_tiles;
+    m.key_groups = 1, m.row_tiles = s.pre_row_tiles, m.heads = x.Hkv, m.parts = s.pre_parts, m.tiles_a_part = s.pre_tiles;
     m.part_o = a.pre_o, m.part_ml = a.pre_ml;
     const unsigned tiles = (unsigned)(s.pre_row_tiles * x.Hkv * s.pre_parts);
     DS2_TRY(f16 ? launch_masked_f16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st) : launch_masked_bf16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st));
