@@ -150,7 +150,7 @@ def test_workspaces_hold_their_parts(lib):
                         rows, group = B * T * G * H, 64 if T * G > 16 else 16
                         streams = B * H * -(-T * G // 16)
                         segments = (1024 + streams) * group * (D + 2) * 4 + streams * 8
-                        parts = -(-P // 64) * rows * (D + 2) * 4
+                        parts = -(-P // 32) * rows * (D + 2) * 4                     # a part of the prefix is 32 keys or more
                         assert 0 <= n <= segments + parts + 256, (D, B, T, G, H, C_, P, n)
     for D in (8, 72, 128, 256):
         for B, Lq, Lk, G, H in ((1, 1, 1, 1, 1), (1, 77, 40000, 2, 2), (3, 4096, 4096, 4, 1), (2, 1, 1 << 20, 8, 4)):
