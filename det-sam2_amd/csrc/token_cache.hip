@@ -92,7 +92,8 @@ struct ReadArgs {
 
 // One thread turns 8 codes into 8 values, four times: the stores of a wave are 1 KB side by side at 16 bits.  The frames above: 89 MB
 // in 13.9 us, 6.4 TB/s (with 16 codes a thread, whose stores leave gaps of 16 bytes between lanes, 15.1); the ragged prompts back, one
-// tensor: 62 MB in 14.8 us (16.4).
+// tensor: 62 MB in 14.8 us (16.4).  Stores past the caches would make that 11.2, but the kernel that takes the values next would lose more
+// (read and copy of 50 MB: 29.6 us so, 32.4 past the caches).
 template <int TYPE, int FORMAT>
 __global__ __launch_bounds__(256) void k_cache_read(ReadArgs a) {
   ds2_ask_args(a);
