@@ -91,7 +91,7 @@ __device__ __forceinline__ void ds2_load_bytes(unsigned* to, __amdgpu_buffer_rsr
 }
 // rows [0, n) of a tensor as a buffer
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ds2_rows(const uint8_t* p, int64_t at, unsigned stride, int n, int row_bytes) {
-  const int bytes = n > 0 ? (int)(min(n, 32) - 1) * (int)stride + row_bytes : 0;
+  const int bytes = ((min(n, 32) - 1) * (int)stride + row_bytes) & ~((n - 1) >> 31);       // 0 behind the end, without a branch
   return __builtin_amdgcn_make_buffer_rsrc((void*)(p + at * stride), 0, bytes, 0x00020000);
 }
 
