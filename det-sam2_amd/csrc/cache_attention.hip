@@ -33,9 +33,13 @@ Split split_of(const ds2_cache_attention_args& a) {
   const bool whole = units <= std::max<int64_t>(4, std::min<int64_t>(16, s.streams / 32));
   s.shares = whole ? 0 : (int)std::min<int64_t>(256 * cache_residents(a.D), s.streams * (units + 1));
   if (a.prefix_len) {
-    // From 64 rows a key head on, the prefix is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve
-    // 256 rows (16-bit caches whose rows follow each other at one stride).
-    s.tiled = a.format == DS2_CACHE_PLAIN && all_rows >= 64 && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
+    // A long prefix of many rows is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve 256 rows (16-bit
+    // caches whose rows follow each other at one stride).  It costs a launch and more parts to join, so the product has to be large.
+    // 8 key heads, prompt kernel / this one: D = 64, 128 rows behind 32768 tokens 40 / 46 us, 256 behind 8192 31 / 28; D = 128, 128
+    // behind 32768 58 / 69, 256 behind 8192 (and up to 512 tokens each) 57 / 50; D = 256, 64 behind 32768 78 / 96, 128 behind 8192 49 / 50,
+    // 256 behind 2000 47 / 33.
+    const double product = (double)a.Hkv * all_rows * a.prefix_len * a.D;
+    s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 && a.D <= 128 ? 3.0e9 : 1.8e9) && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
     if (s.tiled) {
       s.pre_row_tiles = (int)cdiv64(all_rows, masked_rows(a.D, 1));
       const int tiles = cdiv(a.prefix_len, masked_tile(a.D));

@@ -26,8 +26,8 @@ SPLITS = [  # B, T, Hq, Hkv, D, C, P, cap, slopes, formats
     (3, 2, 16, 2, 256, 30, 31, 0.0, True, "mxfp8 mxfp4"),               # prefix chunks of 32 keys and their ends
     (3, 2, 16, 2, 256, 30, 32, 15.0, False, "mxfp8"),
     (3, 2, 16, 2, 96, 30, 33, 0.0, False, "mxfp8 mxfp4"),
-    (6, 1, 8, 1, 128, 30, 127, 0.0, False, "plain mxfp8"),              # 48 rows: not the kernel of prompts
-    (16, 1, 16, 2, 128, 40, 300, 0.0, False, "plain"),                  # 128 rows: the kernel of prompts
+    (6, 1, 8, 1, 128, 30, 127, 0.0, False, "plain mxfp8"),              # 48 rows
+    (16, 1, 16, 2, 128, 40, 300, 0.0, False, "plain"),                  # 128 rows of the prefix
     (16, 1, 16, 2, 96, 600, 65, 0.0, True, "plain"),                    # ... with a bias, and shares
     (9, 2, 16, 2, 64, 20, 70, 25.0, True, "plain"),                     # ... cap and bias, two tokens, some before the first
     (33, 2, 2, 1, 256, 5, 100, 0.0, False, "plain"),
@@ -46,6 +46,34 @@ def test_cache_attention_on_both_sides_of_its_rules(ops, case, form, kind):  # n
     slopes = torch.exp2(-torch.arange(1, Hq + 1).float() * 8 / Hq) if alibi else None
     want, top, score = cache_reference(x, lens, form, D ** -0.5, cap, slopes, P)
     near(run_cache(ops, x, lens, form, D ** -0.5, cap, slopes, P), want, top, score, kind)
+
+
+LARGE = [  # B, T, Hq, Hkv, D, C, P, cap, slopes: products over a prefix that go to the kernel of whole prompts
+    (8, 16, 16, 2, 64, 40, 13800, 0.0, False),
+    (8, 16, 16, 2, 64, 700, 13800, 0.0, True),
+    (16, 8, 16, 2, 96, 9, 15300, 25.0, False),
+    (8, 16, 16, 2, 128, 17, 11500, 20.0, True),
+    (9, 16, 16, 1, 256, 30, 3200, 0.0, True),
+    (700, 1, 3, 1, 32, 3, 26800, 0.0, False),
+]
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: "x".join(map(str, c[:7])))
+def test_a_large_product_over_a_prefix(ops, case, kind):  # noqa: F811
+    B, T, Hq, Hkv, D, C, P, cap, alibi = case
+    g = torch.Generator().manual_seed(sum(case[:7]))
+    x = cache_case(g, B, T, Hq, Hkv, D, C, P, "plain", kind)
+    lens = torch.tensor(lengths(B, C), dtype=torch.int32)
+    slopes = torch.exp2(-torch.arange(1, Hq + 1).float() * 8 / Hq) if alibi else None
+    got = run_cache(ops, x, lens, "plain", D ** -0.5, cap, slopes, P)
+    some = torch.arange(0, B, max(1, B // 8))                               # (the reference of some sequences)
+    few = {**x, **{n: x[n][some] for n in ("q", "k", "v")}}
+    want, top, score = cache_reference(few, lens[some], "plain", D ** -0.5, cap, slopes, P)
+    near(got[some.to(DEV)], want, top, score, kind)
+    if D == 256:                                                            # the same prefix, its tokens 2 MB apart
+        y = {**x, "pk": far(x["pk"], (1 << 20) - 8, 1), "pv": far(x["pv"], (1 << 20) - 64, 1)}
+        assert torch.equal(run_cache(ops, y, lens, "plain", D ** -0.5, cap, slopes, P), got)
 
 
 @pytest.mark.parametrize("form,D", [("plain", 64), ("plain", 256), ("mxfp8", 128)])
@@ -131,7 +159,7 @@ def test_offsets_of_a_cache_beyond_32_bits(ops):  # noqa: F811
     assert torch.equal(run_cache(ops, y, lens, "plain", 0.125, 0.0, None, 140), want)
     y = {**x, "pk": far(x["pk"], (1 << 24) - 16, 1), "pv": far(x["pv"], (1 << 24) - 8, 1)}
     assert torch.equal(run_cache(ops, y, lens, "plain", 0.125, 0.0, None, 140), want)
-    q = torch.randn(70, 1, 4, 64, generator=g).to(torch.bfloat16)           # 280 rows: the prefix in the kernel of prompts
+    q = torch.randn(70, 1, 4, 64, generator=g).to(torch.bfloat16)           # 280 rows of the prefix
     x = {**x, "q": q, "k": x["k"].expand(70, 1, 150, 64), "v": x["v"].expand(70, 1, 150, 64)}
     lens = torch.full((70,), 149, dtype=torch.int32)
     want = run_cache(ops, x, lens, "plain", 0.125, 0.0, None, 140)
