@@ -45,7 +45,7 @@ constexpr int masked_rows(int D, int key_groups) { return 256 / masked_value_spl
 constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }   // keys of a tile
 constexpr float LOG2E = 1.44269504088896340736f;
 // How scores become exponents.  LINEAR: distance bias without a cap, by what the products start from; GENERAL: cap and bias, or a scale
-// that the others do not take.  (D = 64, 16 heads, 8190 tokens with a bias: GENERAL 659 TFLOP/s, LINEAR 727, PLAIN without it 726.)
+// or cap that the others do not take.  (D = 64, 16 heads, 8190 tokens with a bias: GENERAL 659 TFLOP/s, LINEAR 727, PLAIN without it 726.)
 enum { MASKED_PLAIN = 0, MASKED_CAP = 1, MASKED_LINEAR = 2, MASKED_GENERAL = 3 };
 
 }  // namespace
@@ -68,7 +68,7 @@ struct MaskedArgs {
 };
 
 static inline int masked_mode(float scale, float cap, const float* slopes) {
-  if (cap > 0.f) return slopes ? MASKED_GENERAL : MASKED_CAP;
+  if (cap > 0.f) return slopes || cap > DS2_CAP_WIDE ? MASKED_GENERAL : MASKED_CAP;
   if (!(scale >= 0x1p-60f)) return MASKED_GENERAL;               // (PLAIN needs a positive scale, LINEAR divides by it)
   return slopes ? MASKED_LINEAR : MASKED_PLAIN;
 }
@@ -309,8 +309,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     return offset;
   };
   // scores -> values whose exponent (base 2) is factor * value + offset: PLAIN and LINEAR the scores themselves; CAP 1 / (1 +
-  // exp(2 x / cap)), as cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)) (no branch, saturates by itself; off by a few 2^-24 of
-  // cap); GENERAL exponents.
+  // exp(2 x / cap)), the variable part of a capped score (ds2_capped); GENERAL exponents.
   constexpr bool DOWN = MODE == MASKED_CAP;                      // the largest exponent has the smallest value
   const float factor = MODE == MASKED_CAP ? -2.f * cap2 : MODE == MASKED_GENERAL ? 1.f : sc;
   auto exponents = [&](f32x16& s, int key0, float offset) {
@@ -320,9 +319,12 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
       return cap2;
     }
     if constexpr (MODE == MASKED_GENERAL) {
-      if (a.cap > 0.f) {
+      if (a.cap > DS2_CAP_WIDE) {
 #pragma unroll
-        for (int y = 0; y < 16; ++y) s[y] = __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[y] * in_cap)), cap2);
+        for (int y = 0; y < 16; ++y) s[y] = ds2_capped_wide(s[y], in_cap, cap2, sc);
+      } else if (a.cap > 0.f) {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) s[y] = ds2_capped(s[y], in_cap, cap2);
       } else {
 #pragma unroll
         for (int y = 0; y < 16; ++y) s[y] *= sc;

@@ -67,6 +67,7 @@ int check(const ds2_attention_masked_args& a) {
   DS2_REQUIRE(a.D >= 8 && a.D <= 256 && a.D % 8 == 0, "attention_masked: head dim %d is not a multiple of 8 up to 256", a.D);
   DS2_REQUIRE(a.type == DS2_TYPE_BF16 || a.type == DS2_TYPE_F16, "attention_masked: bf16 or fp16 expected, got type %d", a.type);
   DS2_REQUIRE(std::isfinite(a.scale) && std::isfinite(a.cap) && a.cap >= 0.f, "attention_masked: scale and cap must be finite, cap not negative");
+  DS2_REQUIRE(a.cap == 0.f || std::fabs(a.scale) <= 1e30f * a.cap, "attention_masked: the cap is too small for the scale");      // (scale / cap is a factor)
   DS2_REQUIRE((!a.q_doc) == (!a.k_doc), "attention_masked: q_doc and k_doc go together");
   DS2_REQUIRE(a.causal || !a.prefix, "attention_masked: a prefix goes with the causal mask");
   DS2_REQUIRE(a.Lk < (1 << 30) && (int64_t)(a.Hq / a.Hkv) * a.Lq < (1ll << 31) - 512, "attention_masked: sequence too long");

@@ -99,7 +99,7 @@ __device__ __forceinline__ void ds2_load_bytes(unsigned* to, __amdgpu_buffer_rsr
 }
 // rows [0, n) of a tensor as a buffer
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ds2_rows(const uint8_t* p, int64_t at, unsigned stride, int n, int row_bytes) {
-  const int bytes = ((min(n, 32) - 1) * (int)stride + row_bytes) & ~((n - 1) >> 31);       // 0 behind the end, without a branch
+  const int bytes = (int)((unsigned)(min(n, 32) - 1) * stride + row_bytes) & ~((n - 1) >> 31);       // 0 behind the end, without a branch
   return __builtin_amdgcn_make_buffer_rsrc((void*)(p + at * stride), 0, bytes, 0x00020000);
 }
 
@@ -287,10 +287,12 @@ struct CacheStream {
       asm volatile("" ::: "memory");
       // ---- weights
       const bool edge = blk + 32 > common;                 // some row may not see all of the block's keys (uniform)
-      if (a.cap > 0.f) {
-        // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap)): no branch, saturates by itself; off by a few 2^-24 of cap
+      if (a.cap > DS2_CAP_WIDE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = cap2 - 2.f * cap2 * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p[j] * in_cap));
+        for (int j = 0; j < 8; ++j) p[j] = ds2_capped_wide(p[j], in_cap, cap2, sc);
+      } else if (a.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = ds2_capped(p[j], in_cap, cap2);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[j] *= sc;

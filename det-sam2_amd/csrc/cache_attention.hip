@@ -86,6 +86,7 @@ int check(const ds2_cache_attention_args& a) {
   DS2_REQUIRE(a.type == DS2_TYPE_BF16 || a.type == DS2_TYPE_F16, "cache_attention: queries are bf16 or fp16, got type %d", a.type);
   DS2_REQUIRE(a.format == DS2_CACHE_PLAIN || a.format == DS2_CACHE_MXFP8 || a.format == DS2_CACHE_MXFP4, "cache_attention: unknown format %d", a.format);
   DS2_REQUIRE(std::isfinite(a.scale) && std::isfinite(a.cap) && a.cap >= 0.f, "cache_attention: scale and cap must be finite, cap not negative");
+  DS2_REQUIRE(a.cap == 0.f || std::fabs(a.scale) <= 1e30f * a.cap, "cache_attention: the cap is too small for the scale");      // (scale / cap is a factor)
   DS2_REQUIRE((int64_t)a.capacity + a.prefix_len < (1ll << 31) - 4096 && a.T < (1 << 20), "cache_attention: too many tokens");
   DS2_REQUIRE((int64_t)a.B * a.T * a.Hq < (1ll << 31) / 256, "cache_attention: too many rows (B T Hq) for one call");
   const Split s = split_of(a);

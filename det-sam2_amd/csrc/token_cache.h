@@ -9,6 +9,7 @@
 #include "../../include/detsam2_hip.h"
 
 #define DS2_CACHE_GROUP 32
+#define DS2_CAP_WIDE 256.f
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -41,6 +42,20 @@ __device__ __forceinline__ float ds2_high16(unsigned w) {
 __device__ __forceinline__ float ds2_cache_scale(unsigned s) {
   const unsigned bits = s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23;
   return __builtin_bit_cast(float, bits);
+}
+
+// Scores x scale under a cap, as exponents of 2: cap tanh(x scale / cap) log2 e.  cap - 2 cap / (1 + exp(2 u)) has no branch and saturates by
+// itself, but is off by a few 2^-24 of the cap whatever u: good for caps up to DS2_CAP_WIDE (2^-14 there, an eighth of half a step of
+// fp16).  Larger caps take the series of tanh below 1/4 (its next term is below 2^-26).
+__device__ __forceinline__ float ds2_capped(float x, float in_cap, float cap2) {
+  return __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * in_cap)), cap2);
+}
+__device__ __forceinline__ float ds2_capped_wide(float x, float in_cap, float cap2, float sc) {
+  const float u = x * in_cap * 0.34657359f, y = u * u;           // in_cap = 2 log2(e) scale / cap
+  const float p = __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  float near = x * sc * p, far = ds2_capped(x, in_cap, cap2);
+  asm volatile("" : "+v"(near), "+v"(far));                      // (both, and a selection: no branch that splits the wave)
+  return y < 0.0625f ? near : far;
 }
 
 // A kernel's arguments are a few lines of memory that no cache of the chip holds when it starts.  Asked for where they are used they

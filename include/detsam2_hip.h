@@ -329,7 +329,8 @@ typedef struct ds2_strided {
  * x[i] [B,T,H,D] (axes b,t,h; type bf16 / fp16 / fp32) -> codes[i] uint8 [B,H,capacity, D or D/2], scales[i] uint8
  * [B,H,capacity,D/32] (axes b,h,token), token t of sequence b at row pos[b] + t.  pos int32 [B]; count int32 [B] or NULL: only the first
  * count[b] tokens of a sequence are written.  A token whose row is not in [0, capacity) is not written; no other row is
- * touched.  D a multiple of 32 up to 4096; rows of x and of codes 16-byte aligned.  x, codes, scales: HOST arrays of n. */
+ * touched.  D a multiple of 32 up to 4096; rows of x and of codes 16-byte aligned; no two rows that are written share memory.  x, codes,
+ * scales: HOST arrays of n. */
 int ds2_op_cache_write(int32_t n, const ds2_strided* x, const ds2_strided* codes, const ds2_strided* scales, int32_t B, int32_t T,
                        int32_t H, int32_t D, int32_t capacity, const int32_t* pos, const int32_t* count, int32_t type,
                        int32_t format, void* stream);
@@ -339,12 +340,14 @@ int ds2_op_cache_read(const ds2_strided* codes, const ds2_strided* scales, const
 
 /* Attention of the last T tokens of every sequence over its cached tokens and over a prefix that all sequences share:
  *   o = sum_j softmax_j(s_j) v_j,  s_j = scale q.k_j, then cap tanh(s_j / cap) where cap > 0, then - slopes[h] (distance of the tokens)
+ * scale and cap finite, |scale| at most 1e30 cap where there is one.
  * q [B,T,Hq,D] (axes b,t,h), bf16 or fp16; k, v [B,Hkv,capacity,D] (axes b,h,token) in `format` (PLAIN: of q's type; MX: codes with
  * k_scales / v_scales); query head h reads key head h / (Hq / Hkv).  lens int32 [B]: tokens of a sequence in the cache, the T new ones
- * among them; new token t sees the prefix and its own tokens up to lens[b] - T + t; where that is negative it sees nothing.
+ * among them (below 0 counts as 0, beyond the capacity as the capacity); new token t sees the prefix and its own tokens up to lens[b] - T + t; where that is negative it sees nothing.
  * prefix_* [Hkv,prefix_len,D] (axes -,h,token; s0 is not used), or prefix_len = 0.  slopes fp32 [Hq] or NULL.  Rows that see nothing are
  * zero.  out [B,T,Hq,D] contiguous, q's type.  D = 32, 64, 96, 128 or 256; all rows 16-byte aligned (scales: any).
- * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), which goes by the sizes alone. */
+ * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), 16-byte aligned, which goes by the sizes alone;
+ * two calls that may run at once need two of them.  The stream is the caller's, the device the current one; nothing synchronises. */
 typedef struct ds2_cache_attention_args {
   int32_t B, T, Hq, Hkv, D, capacity, prefix_len, type, format;
   float scale, cap;
@@ -357,12 +360,13 @@ int64_t ds2_op_cache_attention_work_bytes(const ds2_cache_attention_args* args);
 int ds2_op_cache_attention(const ds2_cache_attention_args* args, void* work, int64_t work_bytes, void* stream);
 
 /* Masked attention of whole prompts: q [B,Lq,Hq,D], k, v [B,Lk,Hkv,D] (axes b,token,h), bf16 or fp16, out [B,Lq,Hq,D] contiguous.
- * Scores as above; the distance of query i and key j is |q_start[b] + i - j| (q_start int32 [B], NULL = 0).  Query i sees key j if
+ * Scores as above; the distance of query i and key j is |q_start[b] + i - j| (q_start int32 [B], NULL = 0; beyond
+ * +-2^30 counts as that).  Query i sees key j if
  *   j < lens[b]                                   (lens int32 [B] or NULL), and
  *   j <= q_start[b] + i or j < prefix[b]          where causal (prefix int32 [B] or NULL), and
  *   q_doc[b,i] == k_doc[b,j] and k_doc[b,j] >= 0  where documents are given (int32 [B,Lq] / [B,Lk] contiguous, in any order).
  * Rows that see nothing are zero.  D a multiple of 8 up to 256; all rows 16-byte aligned.
- * work: device scratch of ds2_op_attention_masked_work_bytes(args) bytes (0: none needed), which goes by the sizes alone. */
+ * work: as above, of ds2_op_attention_masked_work_bytes(args) bytes. */
 typedef struct ds2_attention_masked_args {
   int32_t B, Lq, Lk, Hq, Hkv, D, type, causal;
   float scale, cap;

@@ -95,6 +95,23 @@ def test_scales_caps_and_slopes_of_every_sign(ops, form, D, scale, cap, slope): 
             near(run_masked(ops, q, k, v, *args), want, top, score, torch.bfloat16)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cap,scale", [(256.0, 0.125), (257.0, 0.125), (257.0, 12.0), (1e4, 0.125), (1e4, 300.0), (3e7, 0.125), (1e30, -0.125)])
+def test_wide_caps(ops, cap, scale, kind):  # noqa: F811
+    """A cap far above the scores changes them little, not at random; scores on both sides of a quarter of it."""
+    g = torch.Generator().manual_seed(4)
+    for form in ("plain", "mxfp8"):
+        x = cache_case(g, 3, 2, 4, 2, 64, 60, 40, form, kind)
+        lens = torch.tensor([60, 17, 3], dtype=torch.int32)
+        want, top, score = cache_reference(x, lens, form, scale, cap, None, 40)
+        near(run_cache(ops, x, lens, form, scale, cap, None, 40), want, top, score, kind)
+    q, k, v, *_ = masked_inputs((2, 80, 90, 4, 2, 64, True, cap, False, None, None, None, None), kind)
+    for slopes in (None, torch.tensor([0.5, 0.1, 0.02, 0.0])):
+        args = (scale, True, cap, slopes, None, torch.tensor([10, 0], dtype=torch.int32), None, None)
+        want, top, score = masked_reference(q, k, v, *args)
+        near(run_masked(ops, q, k, v, *args), want, top, score, kind)
+
+
 PROMPTS = [  # B, Lq, Lk, Hq, Hkv, D, causal, cap, slopes, lens, start, prefix, docs
     (1, 512, 512, 4, 4, 64, True, 0.0, True, None, None, None, None),               # keys in parts, a bias on both sides of the rows
     (1, 300, 300, 2, 2, 128, True, 0.0, False, None, None, None, "sorted"),

@@ -82,7 +82,7 @@ def cache_call(lib, work=FAKE, work_bytes=1 << 40, **c):
 @pytest.mark.parametrize("change,match", [
     (dict(B=-1), "negative size"), (dict(T=-1), "negative size"), (dict(capacity=-1), "negative size"), (dict(prefix_len=-1), "negative size"), (dict(Hkv=0), "share"), (dict(Hq=9), "share"),
     (dict(Hq=1), "share"), (dict(D=72), "head dim"), (dict(D=512), "head dim"), (dict(type=F32), "bf16 or fp16"), (dict(format=4), "unknown format"), (dict(scale=float("inf")), "finite"),
-    (dict(cap=float("nan")), "finite"), (dict(cap=-1.0), "finite"), (dict(capacity=(1 << 31) - 1), "too many tokens"), (dict(T=1 << 20), "too many tokens"), (dict(B=1 << 20, Hq=512), "too many rows"),
+    (dict(cap=float("nan")), "finite"), (dict(cap=-1.0), "finite"), (dict(cap=1e-37), "too small"), (dict(cap=1e-32, scale=-50.0), "too small"), (dict(capacity=(1 << 31) - 1), "too many tokens"), (dict(T=1 << 20), "too many tokens"), (dict(B=1 << 20, Hq=512), "too many rows"),
     (dict(q=strided(512, 512, 64, p=None)), "null pointer"), (dict(lens=None), "null pointer"), (dict(out=None), "null pointer"), (dict(out=FAKE + 8), "16-byte"), (dict(q=strided(512, 512, 60)), "16-byte"),
     (dict(k=strided(0, 0, 0, p=None)), "k is missing"), (dict(k=strided(12800, 6400, 60)), "16-byte"), (dict(v=strided(12800, 6400, 1 << 25)), "out of range"), (dict(v=strided(12800, 6400, -64)), "out of range"),
     (dict(format=1, k_scales=strided(0, 0, 0, p=None)), "missing"), (dict(prefix_len=7, prefix_v=strided(0, 0, 0, p=None)), "missing"),
@@ -121,7 +121,7 @@ def masked_call(lib, work=FAKE, work_bytes=1 << 40, **c):
 
 @pytest.mark.parametrize("change,match", [
     (dict(B=-1), "negative size"), (dict(Lq=-1), "negative size"), (dict(Lk=-1), "negative size"), (dict(Hkv=0), "share"), (dict(Hq=7), "share"), (dict(D=4), "multiple of 8"), (dict(D=264), "multiple of 8"),
-    (dict(type=F32), "bf16 or fp16"), (dict(scale=float("nan")), "finite"), (dict(cap=float("inf")), "finite"), (dict(q_doc=FAKE), "go together"), (dict(causal=0, prefix=FAKE), "causal"),
+    (dict(type=F32), "bf16 or fp16"), (dict(scale=float("nan")), "finite"), (dict(cap=float("inf")), "finite"), (dict(cap=1e-37), "too small"), (dict(q_doc=FAKE), "go together"), (dict(causal=0, prefix=FAKE), "causal"),
     (dict(Lk=1 << 30), "too long"), (dict(Lq=(1 << 31) - 1), "too long"), (dict(B=1 << 24), "too many rows"), (dict(out=None), "16-byte"), (dict(q=strided(0, 0, 0, p=None)), "16-byte"),
     (dict(k=strided(1152, 132, 64)), "16-byte"), (dict(v=strided(1152, 1 << 23, 64)), "out of range"), (dict(k=strided(1152, -128, 64)), "out of range"),
 ])
