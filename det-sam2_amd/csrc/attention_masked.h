@@ -218,15 +218,13 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     if ((t_begin + 1) * KT < len) fetch(second, t_begin + 1);
   }
 
-  // ---- smallest and largest limit and document of the wave and of the workgroup (rows of no document do not widen the range)
-  int lo = limit, hi = limit, dlo = qdoc < 0 ? INT32_MAX : qdoc, dhi = qdoc, dmin = qdoc;
+  // ---- smallest and largest limit and document of the wave and of the workgroup (rows of no document do not widen the range).  Limits
+  // ascend with the row; documents need not.
+  const int lo = __builtin_amdgcn_readlane(limit, 0);
+  int hi = __builtin_amdgcn_readlane(limit, 31), dlo = qdoc < 0 ? INT32_MAX : qdoc, dhi = qdoc, dmin = qdoc;
 #pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    lo = min(lo, __shfl_xor(lo, s)), hi = max(hi, __shfl_xor(hi, s)), dmin = min(dmin, __shfl_xor(dmin, s));
-    dlo = min(dlo, __shfl_xor(dlo, s)), dhi = max(dhi, __shfl_xor(dhi, s));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi), dlo = __builtin_amdgcn_readfirstlane(dlo);
-  dmin = __builtin_amdgcn_readfirstlane(dmin), dhi = __builtin_amdgcn_readfirstlane(dhi);
+  for (int s = 1; s < 32; s <<= 1) dmin = min(dmin, __shfl_xor(dmin, s)), dlo = min(dlo, __shfl_xor(dlo, s)), dhi = max(dhi, __shfl_xor(dhi, s));
+  dmin = __builtin_amdgcn_readfirstlane(dmin), dlo = __builtin_amdgcn_readfirstlane(dlo), dhi = __builtin_amdgcn_readfirstlane(dhi);
   if (lane == 0) wg_lim[wave][1] = hi, wg_lim[wave][2] = dlo, wg_lim[wave][3] = dhi;
   __syncthreads();
   int ghi = 0, gdlo = INT32_MAX, gdhi = -1;
@@ -278,9 +276,11 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   int pos_first = pos, pos_last = pos;                           // of the wave's rows
   float tilt = 0.f;
   if constexpr (BIAS) {
+    if (a.row_lens) {
 #pragma unroll
-    for (int s = 1; s < 32; s <<= 1) pos_first = min(pos_first, __shfl_xor(pos_first, s)), pos_last = max(pos_last, __shfl_xor(pos_last, s));
-    pos_first = __builtin_amdgcn_readfirstlane(pos_first), pos_last = __builtin_amdgcn_readfirstlane(pos_last);
+      for (int s = 1; s < 32; s <<= 1) pos_first = min(pos_first, __shfl_xor(pos_first, s)), pos_last = max(pos_last, __shfl_xor(pos_last, s));
+    }
+    pos_first = __builtin_amdgcn_readlane(pos_first, 0), pos_last = __builtin_amdgcn_readlane(pos_last, 31);
     // (a bias of 2^40 a token leaves the nearest key alone like any larger one: no division overflows)
     if constexpr (MODE == MASKED_LINEAR) slope = fmaxf(-0x1p100f * sc, fminf(slope, 0x1p100f * sc)), tilt = slope / sc;
   }
