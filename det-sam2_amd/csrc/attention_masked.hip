@@ -43,7 +43,8 @@ Plan plan_of(const ds2_attention_masked_args& a) {
   p.parts = p.key_groups = 1;
   for (int kg = 1; kg <= (a.D <= 128 ? 2 : 1); ++kg) {
     const int64_t whole = cdiv64(rows, masked_rows(a.D, kg)) * p.heads;
-    for (int n = 1; n <= (whole < 256 ? std::max(1, std::min(p.tiles / 2, 64)) : 1); ++n) {
+    const int most = whole < 256 ? std::max(1, std::min(p.tiles / 2, 64)) : 1;
+    for (int n = 1; n <= most; n += 1 + n / 8) {
       const double longest = (double)cdiv(p.tiles, n) * (masked_tile(a.D) / 32) / kg;
       const double on_cu = seen < 1 ? whole * n / 256.0 : (double)cdiv64(whole * n, 256);
       const double steps = std::max(longest, longest * seen * on_cu * (a.D <= 64 && on_cu > 1 ? 0.81 : 1));

@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <tuple>
 #include <vector>
@@ -413,23 +414,27 @@ const int32_t* ints(const c10::optional<Tensor>& t, at::IntArrayRef shape, const
 void no_overlap(const Tensor& t, const char* name) {
   // every element of a written tensor has a place of its own: a broadcast axis, or strides that cross, would not
   int64_t need = 1;
-  std::vector<std::pair<int64_t, int64_t>> ax;
-  for (int64_t i = 0; i < t.dim(); ++i)
-    if (t.size(i) > 1) ax.emplace_back(t.stride(i), t.size(i));
-  std::sort(ax.begin(), ax.end());
-  for (const auto& x : ax) {
-    TORCH_CHECK(x.first >= need, "det_sam2: elements of ", name, " overlap in memory");
-    need = x.first * (x.second - 1) + need;
+  std::array<std::pair<int64_t, int64_t>, 4> ax;
+  int n = 0;
+  for (int64_t i = 0; i < t.dim() && n < 4; ++i)
+    if (t.size(i) > 1) ax[n++] = {t.stride(i), t.size(i)};
+  std::sort(ax.begin(), ax.begin() + n);
+  for (int i = 0; i < n; ++i) {
+    TORCH_CHECK(ax[i].first >= need, "det_sam2: elements of ", name, " overlap in memory");
+    need = ax[i].first * (ax[i].second - 1) + need;
   }
 }
 int64_t code_bytes(int32_t format, int64_t D) { return format == DS2_CACHE_MXFP4 ? D / 2 : D; }
+// lead axes and a last one
+void want_rows(const Tensor& t, at::IntArrayRef lead, int64_t last, const char* what, const char* name) {
+  bool same = t.dim() == (int64_t)lead.size() + 1 && t.size(-1) == last;
+  for (size_t i = 0; same && i < lead.size(); ++i) same = t.size(i) == lead[i];
+  TORCH_CHECK(same, "det_sam2: ", what, name, " must be ", lead, " and ", last, " in the last dimension, got ", t.sizes());
+}
 void want_codes(const Tensor& c, const Tensor& s, at::IntArrayRef lead, int64_t D, int32_t format, const char* name) {
   TORCH_CHECK(c.scalar_type() == at::kByte && s.scalar_type() == at::kByte, "det_sam2: codes and scales of ", name, " must be uint8");
-  std::vector<int64_t> cs(lead.begin(), lead.end()), ss(lead.begin(), lead.end());
-  cs.push_back(code_bytes(format, D));
-  ss.push_back(D / 32);
-  TORCH_CHECK(c.sizes() == at::IntArrayRef(cs), "det_sam2: codes of ", name, " must be ", at::IntArrayRef(cs), ", got ", c.sizes());
-  TORCH_CHECK(s.sizes() == at::IntArrayRef(ss), "det_sam2: scales of ", name, " must be ", at::IntArrayRef(ss), ", got ", s.sizes());
+  want_rows(c, lead, code_bytes(format, D), "codes of ", name);
+  want_rows(s, lead, D / 32, "scales of ", name);
 }
 
 // new rows k (and v) [B,T,H,D] -> codes uint8 [B,H,C,D or D/2], scales uint8 [B,H,C,D/32], in place, at rows pos[b] + t
@@ -478,7 +483,7 @@ Tensor cache_read(const Tensor& codes, const Tensor& scales, const c10::optional
   return out;
 }
 
-Tensor scratch(int64_t bytes, const Tensor& like) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+Tensor scratch(int64_t bytes, const Tensor& like) { return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
 // q [B,T,Hq,D] over k, v [B,Hkv,C,...] and the shared prefix [Hkv,P,...] -> [B,T,Hq,D]
 Tensor cache_attention(const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& k_scales,
@@ -503,9 +508,7 @@ Tensor cache_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (mx) want_codes(t, *s, lead, D, a.format, name);
     else {
       TORCH_CHECK(t.scalar_type() == q.scalar_type(), "det_sam2::cache_attention: ", name, " must be of q's type");
-      std::vector<int64_t> want(lead.begin(), lead.end());
-      want.push_back(D);
-      TORCH_CHECK(t.sizes() == at::IntArrayRef(want), "det_sam2::cache_attention: ", name, " must be ", at::IntArrayRef(want), ", got ", t.sizes());
+      want_rows(t, lead, D, "", name);
     }
   };
   rows(k, k_scales, {B, Hkv, C}, "k");
