@@ -31,9 +31,9 @@
 //    share's part of a stream is a segment; k_attn_join joins a stream's segments with fp32 weights.  Beginning a stream costs about as
 //    much as a unit (queries, lengths, the first loads, the join of the waves): each counts one unit more than its keys.  Short streams
 //    get a workgroup each (cache_attention.hip has the rule).
-//  * The shared prefix is one matrix of keys for ALL rows B T G of a key head: it is read once, not once per sequence.  Workgroups of 4 waves
-//    hold different rows over the same keys, in one launch with the sequences' own; a large product over a 16-bit prefix goes to
-//    the kernel of whole prompts instead.
+//  * The shared prefix is one matrix of keys for ALL rows B T G of a key head: it comes from HBM once, not once per sequence.  Its
+//    workgroups are in one launch with the sequences' own; a large product over a 16-bit prefix goes to the kernel of whole prompts
+//    instead.
 //
 // Measured: 32 sequences of 8192 tokens, 8 key heads of 128: 16 bits 191 us, 5.6 TB/s of cache; 8 bits 108 us, 5.1 TB/s; 4 bits 66 us, 4.3
 // TB/s (64 sequences, heads of 64: 186, 107, 74 us).  A large copy makes 4.9 TB/s, a sum over a large tensor 6.0.  Ragged, 65 to 8192

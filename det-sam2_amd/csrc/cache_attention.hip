@@ -21,25 +21,31 @@ struct Split {
 Split split_of(const ds2_cache_attention_args& a) {
   Split s{};
   const int64_t G = a.Hq / a.Hkv, rows = a.T * G, all_rows = a.B * rows;
-  s.by_rows = rows > cache_rows(a.D, false);
+  // The waves of a workgroup take different rows over the same keys, or every 16 rows have a workgroup whose waves split the keys.  The
+  // first reads a cache once; the second leaves no wave without rows, and what it reads again are codes.  4 streams of 24 rows x 17,
+  // D = 128, 4000 tokens, first / second: 16 bits 44 / 53 us, 8 bits 34 / 36, 4 bits 31 / 27; 8 heads of 64 rows, D = 128, 8000 tokens:
+  // 57 / 85, 51 / 53, 45 / 38; 32 x 8 of 20 rows, 600 tokens: 28 / 29, 28 / 19, 26 / 17.
+  s.by_rows = rows > (a.format == DS2_CACHE_PLAIN ? 16 : a.format == DS2_CACHE_MXFP8 ? 32 : 64);
   s.own_rows = cache_rows(a.D, s.by_rows);
   s.own_groups = (int)cdiv64(rows, s.own_rows);
   s.streams = (int64_t)a.B * a.Hkv * s.own_groups;
   // A workgroup for every stream, or equal shares of all keys, as many as the chip holds workgroups.  Streams of one unit or two are not
   // worth the join; the more streams there are, the less the longest one stands out and the longer a stream may be (uniform 8-bit
   // D = 128, a workgroup a stream against shares: 64 streams of 512 keys 13.3 / 16.5 us, of 1024 17.4 / 18.0 and ragged 17.9 / 15.9;
-  // 256 streams of 1024 22.1 / 25.5; 1024 of 2048 98.5 / 114).
+  // 256 streams of 1024 22.1 / 25.5; 1024 of 2048 98.5 / 114).  Waves over the same keys do not share them out: 8 streams of 497 tokens
+  // and 24 rows 20 us whole, 14 in shares.  A stream has at most 128 shares, whose join is as long as their keys (one stream of 100000
+  // tokens: 15 us, 24 in 1024 shares).
   const int64_t units = cdiv64(a.capacity, CACHE_UNIT);
-  const bool whole = units <= std::max<int64_t>(4, std::min<int64_t>(16, s.streams / 32));
-  s.shares = whole ? 0 : (int)std::min<int64_t>(256 * cache_residents(a.D), s.streams * (units + 1));
+  const bool whole = units <= std::max<int64_t>(s.by_rows ? 1 : 4, std::min<int64_t>(16, s.streams / 32));
+  s.shares = whole ? 0 : (int)std::min<int64_t>(std::min<int64_t>(256 * cache_residents(a.D), 128 * s.streams), s.streams * (units + 1));
   if (a.prefix_len) {
     // A long prefix of many rows is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve 256 rows (16-bit
     // caches whose rows follow each other at one stride).  It costs a launch and more parts to join, so the product has to be large.
-    // 8 key heads, prompt kernel / this one: D = 64, 128 rows behind 32768 tokens 40 / 46 us, 256 behind 8192 31 / 28; D = 128, 128
-    // behind 32768 58 / 69, 256 behind 8192 (and up to 512 tokens each) 57 / 50; D = 256, 64 behind 32768 78 / 96, 128 behind 8192 49 / 50,
-    // 256 behind 2000 47 / 33.
+    // 8 key heads, prompt kernel / this one: D = 64, 128 rows behind 32768 tokens 40 / 46 us, 256 behind 8192 30 / 26; D = 128, 128
+    // behind 32768 58 / 70, 64 behind 32768 52 / 45, 256 behind 8192 (and up to 512 tokens each) 57 / 50; D = 256, 32 behind 32768 78 / 67,
+    // 128 behind 8192 49 / 48, 256 behind 8192 66 / 86.
     const double product = (double)a.Hkv * all_rows * a.prefix_len * a.D;
-    s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 && a.D <= 128 ? 3.0e9 : 1.8e9) && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
+    s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 ? 3.0e9 : 1.8e9) && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
     if (s.tiled) {
       s.pre_row_tiles = (int)cdiv64(all_rows, masked_rows(a.D, 1));
       const int tiles = cdiv(a.prefix_len, masked_tile(a.D));
@@ -47,10 +53,11 @@ Split split_of(const ds2_cache_attention_args& a) {
       s.pre_tiles = (int)std::max<int64_t>(a.D <= 64 ? 8 : 4, cdiv64(tiles * whole, 256));
       s.pre_parts = cdiv(tiles, s.pre_tiles);
     } else {
-      s.pre_by_rows = all_rows > cache_rows(a.D, false);
+      // Waves of one workgroup on different rows (see above) where the product is large: 8 key heads of 128, first / second: 64 rows
+      // behind 8192 tokens 20.5 / 18 us, behind 32768 45 / 49; 256 behind 8192, with up to 512 own tokens each, 50 / 53; 8 bits 256 behind
+      // 8000 47 / 39.  A workgroup's keys: a block of 32 for each wave, or for all of them.
+      s.pre_by_rows = all_rows >= 64 && all_rows * a.prefix_len >= (a.format == DS2_CACHE_PLAIN ? 1 << 21 : 1 << 22);
       const int64_t streams = (int64_t)a.Hkv * cdiv64(all_rows, cache_rows(a.D, s.pre_by_rows));
-      // a workgroup's keys: a block of 32 for each wave, or for all of them (7 sequences of 2 tokens behind 1001, 8 heads on one of 256:
-      // chunks of 128 17.6 us, of 32 15.9)
       const int64_t least = s.pre_by_rows ? 32 : CACHE_UNIT;
       s.pre_chunk = (int)std::min<int64_t>(2048, std::max<int64_t>(least, cdiv64(cdiv64(a.prefix_len * streams, 256), least) * least));
       s.pre_parts = (int)cdiv64(a.prefix_len, s.pre_chunk);

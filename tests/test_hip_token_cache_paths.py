@@ -33,6 +33,11 @@ SPLITS = [  # B, T, Hq, Hkv, D, C, P, cap, slopes, formats
     (33, 2, 2, 1, 256, 5, 100, 0.0, False, "plain"),
     (130, 1, 2, 1, 32, 3, 1, 0.0, False, "plain"),                      # a prefix of one token
     (3, 1, 4, 2, 64, 0, 40, 0.0, False, "plain mxfp8"),                 # no room for a token
+    (2, 3, 16, 2, 128, 700, 0, 0.0, True, "plain mxfp8 mxfp4"),         # 24 rows: over the same keys, or 16 and 8
+    (2, 8, 16, 2, 64, 300, 50, 9.0, False, "plain mxfp8 mxfp4"),        # 64 rows
+    (1, 17, 8, 2, 32, 900, 0, 0.0, False, "mxfp8 mxfp4"),               # 68 rows
+    (16, 1, 16, 1, 64, 20, 9000, 0.0, True, "plain mxfp4"),             # 256 rows of a prefix, waves over the same keys
+    (33, 1, 16, 1, 32, 20, 9000, 0.0, False, "mxfp8"),                  # 528 rows, 8 bits
 ]
 
 
@@ -54,6 +59,7 @@ LARGE = [  # B, T, Hq, Hkv, D, C, P, cap, slopes: products over a prefix that go
     (16, 8, 16, 2, 96, 9, 15300, 25.0, False),
     (8, 16, 16, 2, 128, 17, 11500, 20.0, True),
     (9, 16, 16, 1, 256, 30, 3200, 0.0, True),
+    (9, 16, 16, 1, 256, 30, 5100, 0.0, True),
     (700, 1, 3, 1, 32, 3, 26800, 0.0, False),
 ]
 
