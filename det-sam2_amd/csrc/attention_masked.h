@@ -212,7 +212,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
 
   // The first two tiles of an undocumented call are known before the limits of all rows are: they are asked for at once (a tile behind
   // every limit is not used).
-  const int t_begin = part * a.tiles_a_part;
+  int t_begin = part * a.tiles_a_part;
   if (!td && t_begin * KT < len) {
     fetch(tile, t_begin);
     if ((t_begin + 1) * KT < len) fetch(second, t_begin + 1);
@@ -232,7 +232,8 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   for (int w = 0; w < NW; ++w) ghi = max(ghi, wg_lim[w][1]), gdlo = min(gdlo, wg_lim[w][2]), gdhi = max(gdhi, wg_lim[w][3]);
   ghi = __builtin_amdgcn_readfirstlane(ghi), gdlo = __builtin_amdgcn_readfirstlane(gdlo), gdhi = __builtin_amdgcn_readfirstlane(gdhi);
 
-  const int t_end = min((ghi + KT - 1) / KT, (part + 1) * a.tiles_a_part);
+  int t_end = (ghi + KT - 1) / KT;
+  if (!td || a.parts == 1) t_end = min(t_end, t_begin + a.tiles_a_part);
   // next tile at or behind t that may hold a visible pair (the same answer in every wave); t_end: none.  64 tiles are looked at a time,
   // one a lane, and kept.
   int window = -64;
@@ -252,6 +253,10 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     }
     return t_end;
   };
+  if (td && a.parts > 1) {                                       // a part of what lies behind the first tile that counts, not of all keys
+    const int from = next_tile(0), per = (t_end - from + a.parts - 1) / a.parts;
+    t_begin = from + part * per, t_end = min(t_end, t_begin + per);
+  }
   // the one document of the tile that next_tile has just found; -1: several, or keys of none; OTHER: none of the wave's rows
   constexpr int OTHER = -2;
   auto tile_doc = [&](int t) {

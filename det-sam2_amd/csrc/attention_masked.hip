@@ -39,13 +39,17 @@ Plan plan_of(const ds2_attention_masked_args& a) {
   // 28736 in eight parts 175 us, two 332; the 1024 tokens above in one part 39, four 60.
   const double part_us = (double)a.B * a.Lq * a.Hq * a.D * 8 / 4e6, step_us = a.D > 128 ? 1.8 : a.D > 96 ? 1.15 : a.D > 64 ? 1.0 : 0.8;
   const double seen = a.causal && a.Lk ? 1 - 0.5 * std::min(1.0, (double)a.Lq / a.Lk) : 1;      // of all pairs
+  // Tiles of a row.  How long documents are is known to the device only, which splits what a tile of rows can see; half of all keys is
+  // between one document and many (6073 tokens in 7 documents, 2 heads of 64: planned for all 66 us, half 38; 4274 in 2, 4 heads: 41,
+  // 36, and 61 for a quarter).
+  const int reach = a.q_doc ? cdiv(p.tiles, 2) : p.tiles;
   double best = 1e300;
   p.parts = p.key_groups = 1;
   for (int kg = 1; kg <= (a.D <= 128 ? 2 : 1); ++kg) {
     const int64_t whole = cdiv64(rows, masked_rows(a.D, kg)) * p.heads;
-    const int most = whole < 256 ? std::max(1, std::min(p.tiles / 2, 64)) : 1;
+    const int most = whole < 256 ? std::max(1, std::min(reach / 2, 64)) : 1;
     for (int n = 1; n <= most; n += 1 + n / 8) {
-      const double longest = (double)cdiv(p.tiles, n) * (masked_tile(a.D) / 32) / kg;
+      const double longest = (double)cdiv(reach, n) * (masked_tile(a.D) / 32) / kg;
       const double on_cu = seen < 1 ? whole * n / 256.0 : (double)cdiv64(whole * n, 256);
       const double steps = std::max(longest, longest * seen * on_cu * (a.D <= 64 && on_cu > 1 ? 0.81 : 1));
       const double us = steps * step_us * (kg > 1 ? 1.25 : 1) + (n > 1 ? 7 + n * part_us : 0);

@@ -127,6 +127,8 @@ PROMPTS = [  # B, Lq, Lk, Hq, Hkv, D, causal, cap, slopes, lens, start, prefix, 
     (1, 64, 2500, 2, 1, 128, True, 0.0, True, [2400], [2436], [100], None),
     (2, 9, 1500, 8, 8, 40, False, 0.0, False, [1500, 700], None, None, None),
     (1, 1200, 100, 1, 1, 64, True, 0.0, True, None, [-500], None, None),            # many rows before the first key
+    (1, 5100, 5100, 1, 1, 64, True, 0.0, False, None, None, None, "sorted"),        # documents in parts
+    (1, 4100, 4100, 1, 1, 128, False, 0.0, True, [4000], None, None, "mixed"),
     (1, 2100, 33, 8, 1, 32, False, 0.0, True, None, [7], None, None),
     (5, 1, 70, 16, 4, 64, True, 0.0, False, [70, 1, 0, 33, 64], [69, 0, 3, 40, 63], None, None),
 ]
