@@ -19,10 +19,12 @@
 //  * causal, prefix and length masks are one number a row: the keys it sees are those below `limit`.  Tiles beyond every row's limit are
 //    not visited, steps below every row's limit are not masked.  Documents: a small kernel notes the smallest and largest document of
 //    each key tile; a wave-wide vote over 64 tiles at a time finds the tiles that can hold a visible pair.
-//  * The running maximum is raised only by more than 2^8: the weights stay below 2^8 and the rescaling of O is rare.
+//  * The running reference of a row is raised only when a weight would exceed a fixed power of 2 (DS2_LIMIT): the weights stay bounded and the
+//    rescaling of O is rare.
 //  * Where 256 rows a workgroup would leave CUs idle or unevenly loaded, the eight waves hold 128 rows twice (KG = 2): each takes every
 //    other step of the tiles, and the two halves are joined through LDS at the end (attention_masked.hip has the rule).
-//  * Weights are rounded to the operands' 16-bit type before the value product: one rounding of half a step, like the output's own.
+//  * Weights are rounded to the operands' 16-bit type before the value product: one rounding of half a step, like the output's own (fp16:
+//    down to 2^-25 of the row's largest weight; DS2_SHIFT).
 //
 // Measured (16-bit operands in, TFLOP/s over the visible pairs): D = 128, 32 over 8 heads, 8192 tokens: full 967, causal 945, capped
 // 830, distance bias 895; a plain library product of 16-bit matrices makes 1096 on the same card.  D = 64, 16 heads, 8190 tokens: 730,
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   const unsigned k_lane = c * KROW + h * 16;
   const unsigned v_lane = (4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4 & 1) * 16 + 4 * (lane & 3) + d0) * 2;
   f32x16 o[DB];
-  float m, l;
+  float m, l;                                                    // reference and sum of the weights
   auto clear = [&]() {
 #pragma unroll
     for (int x = 0; x < DB; ++x)
@@ -364,10 +366,14 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     float top = s[0];
 #pragma unroll
     for (int y = 1; y < 16; ++y) top = DOWN ? fminf(top, s[y]) : fmaxf(top, s[y]);
-    top = __builtin_fmaf(top, factor, offset);
-    if (__any(top > m + 8.f)) {
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top);
+    float off = offset - fmaxf(m, -3e38f);
+    if (__any(__builtin_fmaf(top, factor, off) > DS2_LIMIT<F16>)) {
+      float t = __builtin_fmaf(top, factor, offset);
+      t = fmaxf(t, __shfl_xor(t, 32));
+      float mn = fmaxf(m, t - DS2_SHIFT<F16>);
+      float most = __builtin_fmaf(top, factor, offset - mn);
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (most > DS2_LIMIT<F16>) mn = fmaxf(m, t);                  // (scores so large that fp32 does not hold the difference)
       const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       l *= al;
 #pragma unroll
@@ -375,10 +381,11 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
 #pragma unroll
         for (int y = 0; y < 16; ++y) o[x][y] *= al;
       m = mn;
+      off = offset - fmaxf(m, -3e38f);
     }
+    return off;
   };
-  auto weights = [&](f32x16& s, float offset) {
-    const float off = offset - (m == -INFINITY ? 0.f : m);
+  auto weights = [&](f32x16& s, float off) {                     // (off: what raise has returned)
 #pragma unroll
     for (int y = 0; y < 16; ++y) {
       s[y] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[y], factor, off));
@@ -434,11 +441,11 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
             if (doc0 == OTHER) offset = -INFINITY;                // (no weight; a step that is left out would tear the pipeline)
             else hide(s, key0, buf, half);
           }
-          raise(s, offset);
+          const float off = raise(s, offset);
           f32x16 n;
           const int key1 = st + 1 < ST ? key0 + 32 : t1 * KT + kg * 32;          // (behind the last tile: not used)
           const float offset1 = scores(n, st + 1 < ST ? buf : next, st + 1 < ST ? half + 1 : kg, key1);
-          weights(s, offset);
+          weights(s, off);
           const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
 #pragma unroll
           for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
@@ -493,8 +500,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           float offset = scores(s, 0, half, key0);
           offset = exponents(s, key0, offset);
           if (edge) hide(s, key0, 0, half);
-          raise(s, offset);
-          weights(s, offset);
+          weights(s, raise(s, offset));
           if (edge) {
 #pragma unroll 1
             for (int key = 0; key < 32; ++key) {

@@ -20,12 +20,13 @@
 //    At D = 256 two waves share the rows and keys, each with half of the values (both compute the scores).
 //  * The loads are buffer loads: offsets are lane constants, the block is the descriptor's (scalar) base, keys behind the end cost
 //    nothing.  The next block's keys are asked for as soon as this one's scores are done, its values after the value product.
-//  * The running maximum is raised only when a score exceeds it by more than 2^8: the weights stay below 2^8, the sums are fp32, and
-//    the cross-lane reduction and the rescaling of O leave the loop after the first blocks.
+//  * The running reference of a row is raised only when a weight would exceed a fixed power of 2 (DS2_LIMIT): the weights stay bounded, the
+//    sums are fp32, and the cross-lane reduction and the rescaling of O leave the loop after the first blocks.
 //  * Quantised codes are converted with their scale into bf16, which holds code * 2^e exactly (at most 4 significant bits and an 8-bit
 //    exponent).  fp16 queries become TWO bf16 operands whose sum is exact; the weights become two bf16 operands (16 significant
 //    bits) wherever the values are bf16: the matrix pipe idles in this kernel, the second product is free, and the result carries no
-//    rounding but the output's.  fp16 caches: the weights are one fp16 operand (11 bits, the output's own precision).
+//    rounding but the output's.  fp16 caches: the weights are one fp16 operand (11 bits, the output's own precision, down to 2^-25
+//    of the row's largest; DS2_SHIFT).
 //  * The work is cut into equal shares, not into sequences: all keys of all (sequence, key head) streams are laid end to end in units of 128
 //    and every workgroup takes the same number of units, wherever streams begin and end (the lengths are read on the device).  A
 //    share's part of a stream is a segment; k_attn_join joins a stream's segments with fp32 weights.  Beginning a stream costs about as
@@ -161,7 +162,7 @@ struct CacheStream {
 
   u32x4 q[KS], ql[QLO ? KS : 1];
   f32x4 o[E];
-  float m, l;
+  float m, l;               // reference and sum of the weights
   float slope;              // * log2 e
   int pos, sees;            // position of the lane's row and how many keys it sees, both counted in the keys of this stream
   unsigned vw[8][VW], kscale[2][SG], vscale[8];
@@ -307,17 +308,18 @@ struct CacheStream {
           if (blk + (j < 4 ? 0 : 12) + 4 * g + j >= sees) p[j] = -INFINITY;
       }
       float top = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
-      if (__any(top > m + 8.f)) {
+      if (__any(top - fmaxf(m, -3e38f) > DS2_LIMIT<F16>)) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top);
+        float mn = fmaxf(m, top - DS2_SHIFT<F16>);
+        if (top - mn > DS2_LIMIT<F16>) mn = top;           // (scores so large that fp32 does not hold the difference)
         const float al = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         l *= al;
 #pragma unroll
         for (int t = 0; t < E; ++t) o[t] *= al;
         m = mn;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = fmaxf(m, -3e38f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         p[j] = __builtin_amdgcn_exp2f(p[j] - ref);

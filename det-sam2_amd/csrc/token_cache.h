@@ -19,6 +19,18 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
+// The weights of a row are powers of 2 relative to a running reference.  It is raised when one of them would exceed 2^DS2_LIMIT, and then set so
+// that the row's largest weight is 2^DS2_SHIFT: sums and unnormalised results carry that factor, the reference that goes with them says
+// so.  bf16 has the exponents of fp32 and needs none.  fp16 ends at 2^16 and loses bits below 2^-14: with weights of 2^11 to 2^15 for
+// the largest, 11 bits remain down to 2^-25 of it, and below that no weight is off by more than 2^-36 of it.  (References at the largest score and a
+// limit of 2^8: 11 bits down to 2^-14, nothing at all below 2^-25.  Where the largest weight falls on a value of zero and the others are e^-17.5 of
+// it, the row was off by 10 to 40 half steps of the output.)  Raising after 2^4 and not 2^8 costs 3 % where
+// a bias lets the scores climb from key to key (4096 rows over 28736 keys, D = 64: 182 -> 187 us); elsewhere it is rare after a row's first keys.
+template <bool F16>
+constexpr float DS2_SHIFT = F16 ? 11.f : 0.f;
+template <bool F16>
+constexpr float DS2_LIMIT = F16 ? 15.f : 8.f;
+
 #ifdef __HIPCC__
 // two fp32 values -> two 16-bit values in a word (round to nearest even)
 template <bool F16>

@@ -1,0 +1,88 @@
+"""Attention over a cache and masked attention where precision is decided: rows whose mass is one key and a long tail, weights of 16 bits,
+distances far from the keys.  Plain forms: test_hip_token_cache.py.
+
+Bounds, of |got - want|, with u half a step of the output's type (bf16 2^-8, fp16 2^-11) and w_j the weights over their sum:
+  * u |want|: the output's own rounding;
+  * sum_j r_j |v_j|, r_j what the rounding of a weight takes from it: u w_j where weights are one operand of the output's type, for fp16 not
+    below half its smallest step, 2^-25, relative to the largest weight that an operand holds, 2^11 (the kernels scale
+    fp16 weights by that, so that the largest of a row, up to 2^4 over the running maximum, is still finite): 2^-36 of the row's largest
+    weight; 2^-16 w_j where weights are two bf16 operands (half a step of a half step, 2^-8 2^-8);
+  * scores: with n elements of q that are not zero the fp32 score is off by at most (n + 8) 2^-24 times the sum of its terms' sizes, the
+    exponent's products and sums by a few 2^-24 of the score: 2 (n + 8) 2^-24 score, relative to every weight;
+  * sums of N keys in fp32, 32 keys to a product, 8 roundings at most within one: (N / 4 + 64) 2^-24 of sum_j w_j |v_j|;
+  * 2^-24 for outputs that are subnormal in fp16."""
+import math
+
+import pytest
+import torch
+
+from test_hip_token_cache import cache_reference, masked_reference, ops, run_cache, run_masked  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def within(got, want, top, score, kind, weights, nonzero, keys, tail=0.0):
+    """`weights`: relative rounding of a weight; `tail`: what the smallest weights may lose, sum_j |v_j| 2^-36 at most"""
+    u = torch.finfo(kind).eps / 2
+    assert bool(torch.isfinite(want).all())
+    bound = u * want.abs() + (weights + 2 * (nonzero + 8) * 2.0 ** -24 * score.unsqueeze(-1) + (keys / 4 + 64) * 2.0 ** -24) * top + tail + 2.0 ** -24
+    off = (got.double().cpu() - want).abs() / bound
+    assert float(off.nan_to_num(math.inf).max()) <= 1.0, float(off.nan_to_num(math.inf).max())
+
+
+# ---- one key far above all others, whose value is zero: the row's result is the tail's -----------------------------------------------
+
+def sink(g, q_lead, k_lead, axis, N, D, at, gap):
+    """Queries along the first axis; keys of score 0 to 1, one of `gap` with a value of zero; values from 20 to 60."""
+    q = torch.zeros(*q_lead, D)
+    q[..., 0] = 1
+    k, v = torch.zeros(*k_lead, D), 20 + 40 * torch.rand(*k_lead, D, generator=g)
+    k[..., 0] = torch.rand(*k_lead, generator=g)
+    k.select(axis, at)[..., 0] = gap
+    v.select(axis, at)[...] = 0
+    return q.half(), k.half(), v.half()
+
+
+GAPS = [11.0, 15.0, 17.5, 19.0]
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("D,Lq,Lk,at,mode", [(64, 40, 900, 5, "plain"), (128, 300, 3001, 0, "plain"), (256, 33, 500, 2, "plain"), (32, 500, 500, 0, "causal"), (96, 130, 700, 9, "cap"),
+                                             (64, 70, 2000, 1, "bias"), (128, 600, 600, 300, "doc"), (64, 4, 9000, 0, "plain")])
+def test_a_tail_far_below_one_key_of_a_prompt(ops, D, Lq, Lk, at, mode, gap):  # noqa: F811
+    g = torch.Generator().manual_seed(D + Lk)
+    q, k, v = sink(g, (1, Lq, 2), (1, Lk, 1), 1, Lk, D, at, gap)
+    slopes = torch.tensor([2.0 ** -14, 2.0 ** -13]) if mode == "bias" else None
+    doc = (torch.arange(Lk) // 300).int().unsqueeze(0) if mode == "doc" else None
+    cap = 200.0 if mode == "cap" else 0.0
+    args = (1.0, mode == "causal", cap, slopes, None, None, None, doc)
+    want, top, score = masked_reference(q, k, v, *args)
+    within(run_masked(ops, q, k, v, *args), want, top, score + (cap and 4 * cap / 10), torch.float16, 2.0 ** -11, 1, Lk, Lk * 60 * 2.0 ** -36)
+
+
+TAILS = [  # B, T, Hq, Hkv, D, C, P, where the far key lies: own tokens, the prefix
+    (1, 1, 2, 1, 64, 400, 0, "own"),                  # a workgroup a stream
+    (2, 1, 4, 2, 128, 3000, 0, "own"),                # shares
+    (2, 5, 8, 2, 32, 3000, 0, "own"),                 # waves on different rows
+    (2, 1, 4, 2, 256, 900, 0, "own"),
+    (2, 1, 4, 2, 96, 60, 500, "prefix"),
+    (2, 1, 4, 2, 64, 500, 60, "own"),
+    (64, 1, 16, 2, 64, 33, 9000, "prefix"),           # the product over the prefix is large: the kernel of whole prompts
+    (64, 1, 16, 2, 64, 33, 9000, "own"),
+    (40, 2, 8, 1, 256, 20, 7600, "prefix"),
+]
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("case", TAILS, ids=lambda c: "x".join(map(str, c)))
+def test_a_tail_far_below_one_key_of_a_cache(ops, case, gap):  # noqa: F811
+    B, T, Hq, Hkv, D, C, P, where = case
+    g = torch.Generator().manual_seed(D + C)
+    q, k, v = sink(g, (B, T, Hq), (B, Hkv, C), 2, C, D, 2, gap if where == "own" else 0.5)
+    _, pk, pv = sink(g, (1,), (Hkv, P), 1, P, D, 2, gap if where == "prefix" else 0.5) if P else (None, torch.zeros(Hkv, 0, D).half(), torch.zeros(Hkv, 0, D).half())
+    x = {"q": q, "k": k, "v": v, "pk": pk, "pv": pv, "ks": None, "vs": None, "pks": None, "pvs": None}
+    lens = torch.full((B,), C, dtype=torch.int32)
+    got = run_cache(ops, x, lens, "plain", 1.0, 0.0, None, P)
+    few = {**x, **{n: x[n][:2] for n in ("q", "k", "v")}}
+    want, top, score = cache_reference(few, lens[:2], "plain", 1.0, 0.0, None, P)
+    within(got[:2], want, top, score, torch.float16, 2.0 ** -11, 1, C + P, (C + P) * 60 * 2.0 ** -36)
