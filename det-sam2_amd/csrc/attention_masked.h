@@ -155,6 +155,10 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     if (a.prefix) n = max(n, a.prefix[b]);
     limit = max(0, min(len, n));
   }
+  // A row before the first key or behind the last has part of every distance in common, which is no part of a softmax: for the bias it stands
+  // at that key, so that no exponent is a small difference of large ones.  (At 10^6 behind the keys with a slope of 1/2 exponents have steps of 1/16.)
+  // Rows behind a shared prefix keep their places: their parts are joined with those of their own keys.
+  if (BIAS && !a.row_lens) pos = max(0, min(pos, len - 1));
   int qdoc = a.q_doc ? a.q_doc[(int64_t)b * a.Lq + i] : 0;
   qdoc = qdoc < 0 ? -2 : qdoc;                                   // of no document: equal to no key's (a key of none is -1 in LDS)
 

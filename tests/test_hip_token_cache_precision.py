@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from test_hip_token_cache import cache_reference, masked_reference, ops, run_cache, run_masked  # noqa: F401
+from test_hip_token_cache import DEV, cache_reference, masked_reference, ops, run_cache, run_masked  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,24 @@ def test_a_tail_far_below_one_key_of_a_cache(ops, case, gap):  # noqa: F811
     few = {**x, **{n: x[n][:2] for n in ("q", "k", "v")}}
     want, top, score = cache_reference(few, lens[:2], "plain", 1.0, 0.0, None, P)
     within(got[:2], want, top, score, torch.float16, 2.0 ** -11, 1, C + P, (C + P) * 60 * 2.0 ** -36)
+
+
+# ---- positions far from the keys: what all keys of a row have in common is no part of a softmax -------------------------------------
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("start,causal", [([10 ** 6, -10 ** 6], False), ([2 ** 30, 12345678], True), ([2 ** 31 - 1, -2 ** 31], False), ([700, -300], False)])
+@pytest.mark.parametrize("D,Lq,Lk", [(64, 50, 400), (128, 200, 300), (256, 7, 2000)])
+def test_queries_far_from_the_keys(ops, D, Lq, Lk, start, causal, cap, kind):  # noqa: F811
+    """The distance of key j is that of the nearest key and what j adds to it, and the first part is the same for all keys of a row."""
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (torch.randn(2, n, h, D, generator=g).to(kind) for n, h in ((Lq, 4), (Lk, 2), (Lk, 2)))
+    slopes = torch.tensor([0.5, 0.1, -0.03, 2.0 ** -8])
+    lens = torch.tensor([Lk, Lk - 90], dtype=torch.int32)
+    at = torch.tensor(start, dtype=torch.int64).clamp(-2 ** 30, 2 ** 30)
+    args = (D ** -0.5, causal, cap, slopes, lens)
+    want, top, _ = masked_reference(q, k, v, *args, at, None, None)
+    score = torch.full(want.shape[:-1], 30.0 + 0.5 * 60 + 0.03 * (Lk + Lq))    # sizes that carry weight: products, bias from the nearest key on
+    got = ops.attention_masked(q.to(DEV), k.to(DEV), v.to(DEV), D ** -0.5, causal, cap, slopes.to(DEV), lens.to(DEV),
+                               torch.tensor(start, dtype=torch.int32, device=DEV), None, None, None)
+    within(got, want, top, score, kind, torch.finfo(kind).eps / 2, D, Lk, Lk * float(v.abs().max()) * 2.0 ** -36)
