@@ -58,8 +58,9 @@ struct MaskedArgs {
   int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;    // bytes
   const float* slopes;
   const int32_t *lens, *q_start, *prefix, *q_doc, *k_doc;
-  const int32_t* row_lens;                  // rows of sequences behind a shared prefix of Lk keys (cache_attention.hip): position i stands at
-  int row_T, row_C;                         // Lk + row_lens[i / row_T] - row_T + i % row_T, row_lens at most row_C; null: at q_start + i
+  const int32_t* row_lens;                  // rows of sequences behind a shared prefix of Lk keys (cache_attention.hip): position i is token i % row_T
+  int row_T, row_C;                         // of sequence i / row_T (B is 1) and stands at Lk + row_lens[sequence] - row_T + token, row_lens at
+                                            // most row_C; null: at q_start + i
   const int2* tile_docs;                    // [B][tiles]: smallest (-1: a key of none among them) and largest document of a tile
   int B, Lq, Lk, Hq, Hkv, G, D, causal;
   float scale, cap;
@@ -144,10 +145,9 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   const int len = a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
   const int start = a.q_start ? max(-(1 << 30), min(a.q_start[b], 1 << 30)) : 0;
   int pos = start + i;
-  if (BIAS && a.row_lens) {
-    const int seq = i / a.row_T;
-    pos = a.Lk + max(0, min(a.row_lens[seq], a.row_C)) - a.row_T + i - seq * a.row_T;
-  }
+  int seq = b, token = i;
+  if (a.row_lens) seq = i / a.row_T, token = i - seq * a.row_T;
+  if (BIAS && a.row_lens) pos = a.Lk + max(0, min(a.row_lens[seq], a.row_C)) - a.row_T + token;
   float slope = BIAS && a.slopes ? a.slopes[hq] * LOG2E : 0.f;
   int limit = len;
   if (a.causal) {
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   // ---- queries
   u32x4 qf[KS];
   {
-    const char* row = a.q + b * a.q_b + (int64_t)i * a.q_t + hq * a.q_h;
+    const char* row = a.q + seq * a.q_b + (int64_t)token * a.q_t + hq * a.q_h;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = 16 * s + 8 * h;

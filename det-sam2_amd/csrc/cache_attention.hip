@@ -40,12 +40,13 @@ Split split_of(const ds2_cache_attention_args& a) {
   s.shares = whole ? 0 : (int)std::min<int64_t>(std::min<int64_t>(256 * cache_residents(a.D), 128 * s.streams), s.streams * (units + 1));
   if (a.prefix_len) {
     // A long prefix of many rows is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve 256 rows (16-bit
-    // caches whose rows follow each other at one stride).  It costs a launch and more parts to join, so the product has to be large.
+    // caches).  It costs a launch and more parts to join, so the product has to be large.
     // 8 key heads, prompt kernel / this one: D = 64, 128 rows behind 32768 tokens 40 / 46 us, 256 behind 8192 30 / 26; D = 128, 128
     // behind 32768 58 / 70, 64 behind 32768 52 / 45, 256 behind 8192 (and up to 512 tokens each) 57 / 50; D = 256, 32 behind 32768 78 / 67,
-    // 128 behind 8192 49 / 48, 256 behind 8192 66 / 86.
+    // 128 behind 8192 49 / 48, 256 behind 8192 66 / 86; one sequence of 64 tokens (256 rows a head, D = 128) behind 32768 77 / 105, of 512
+    // tokens 339 / 736.  (By sizes alone, whatever the queries' strides: the workspace goes by it.)
     const double product = (double)a.Hkv * all_rows * a.prefix_len * a.D;
-    s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 ? 3.0e9 : 1.8e9) && (a.T == 1 || a.q.s0 == a.T * a.q.s1);
+    s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 ? 3.0e9 : 1.8e9);
     if (s.tiled) {
       s.pre_row_tiles = (int)cdiv64(all_rows, masked_rows(a.D, 1));
       const int tiles = cdiv(a.prefix_len, masked_tile(a.D));
@@ -170,7 +171,7 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
   if (s.tiled) {
     MaskedArgs m{};
     m.q = a.q, m.k = (const char*)a.pk, m.v = (const char*)a.pv, m.out = a.out;
-    m.q_t = x.T == 1 ? a.q_b : a.q_t, m.q_h = a.q_h;
+    m.q_b = a.q_b, m.q_t = a.q_t, m.q_h = a.q_h;
     m.k_t = a.pk_c, m.k_h = a.pk_h, m.v_t = a.pv_c, m.v_h = a.pv_h;
     m.slopes = a.slopes, m.row_lens = x.lens, m.row_T = x.T, m.row_C = x.capacity;
     m.B = 1, m.Lq = x.B * x.T, m.Lk = x.prefix_len, m.Hq = x.Hq, m.Hkv = x.Hkv, m.G = a.G, m.D = x.D;

@@ -1,0 +1,17 @@
+"""What the C entries of the token cache and its attention promise about sizes, without a GPU."""
+import ctypes as C
+
+from test_token_cache_host import cache_args, lib, strided  # noqa: F401
+
+
+def test_the_workspace_goes_by_the_sizes_alone(lib):  # noqa: F811
+    """Whatever the strides: a caller sizes it once."""
+    for D in (32, 64, 96, 128, 256):
+        for B, T, G, H in ((64, 2, 4, 2), (2, 64, 8, 1), (1, 512, 4, 2), (1, 1, 8, 8), (16, 16, 2, 8), (300, 3, 1, 2)):
+            for P in (0, 500, 9000, 65536):
+                for C_ in (0, 40, 512, 5000):
+                    sizes = dict(B=B, T=T, Hq=G * H, Hkv=H, D=D, capacity=C_, prefix_len=P)
+                    row = G * H * D
+                    need = {lib.ds2_op_cache_attention_work_bytes(C.byref(cache_args(q=q, **sizes)))
+                            for q in (strided(T * row, row, D), strided(row, B * row, D), strided(0, row, D), strided(2 * T * row, row, D), strided(T * row, D, T * D), strided(0, 0, 0, p=None))}
+                    assert len(need) == 1, (sizes, need)
