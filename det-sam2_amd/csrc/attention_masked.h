@@ -23,8 +23,10 @@
 //    rescaling of O is rare.
 //  * Where 256 rows a workgroup would leave CUs idle or unevenly loaded, the eight waves hold 128 rows twice (KG = 2): each takes every
 //    other step of the tiles, and the two halves are joined through LDS at the end (attention_masked.hip has the rule).
-//  * Weights are rounded to the operands' 16-bit type before the value product: one rounding of half a step, like the output's own (fp16:
-//    down to 2^-25 of the row's largest weight; DS2_SHIFT).
+//  * Weights are rounded to the operands' 16-bit type before the value product, while their sum takes them as they are: half a step of each term
+//    w |v|, like the output's own rounding (fp16: down to 2^-25 of the row's largest weight; DS2_SHIFT).  Two bf16 operands (WIDE) leave 2^-16 and
+//    take up to a fifth more time (8 key heads, 2048 rows a head behind 8192 tokens: D = 64 69 -> 84 us, D = 128 105 -> 127).  A prefix that
+//    sequences share has them, as their own tokens do; whole prompts have one.
 //
 // Measured (16-bit operands in, TFLOP/s over the visible pairs): D = 128, 32 over 8 heads, 8192 tokens: full 967, causal 945, capped
 // 830, distance bias 895; a plain library product of 16-bit matrices makes 1096 on the same card.  D = 64, 16 heads, 8190 tokens: 730,
@@ -77,6 +79,7 @@ static inline int masked_mode(float scale, float cap, const float* slopes) {
 }
 int launch_masked_bf16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
 int launch_masked_f16(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);
+int launch_masked_bf16_wide(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st);        // weights as two operands, one key group
 
 namespace {
 
@@ -94,7 +97,7 @@ __device__ __forceinline__ unsigned not_finite(unsigned w) {
 
 // The register limit keeps accumulators out of the AGPRs.  With them, and a divergent branch in the tile loop, hipcc placed copies into
 // AGPRs in front of the restored lane mask; the loop below has wave-uniform branches only.
-template <bool F16, int DP, int MODE, int KG>
+template <bool F16, int DP, int MODE, int KG, bool WIDE>
 __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs a) {
   ds2_ask_args(a);
   constexpr int NW = 8;                                          // waves (those without rows of their own stage keys for the others)
@@ -402,6 +405,12 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
     for (int y = 0; y < 4; ++y) p[y] = ds2_pack16<F16>(s[8 * kk + 2 * y], s[8 * kk + 2 * y + 1]);
     return p;
   };
+  auto rest = [&](const f32x16& s, const u32x4& p, int kk) {     // WIDE: what that rounding left, as another
+    u32x4 r;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) r[y] = ds2_pack16<F16>(s[8 * kk + 2 * y] - ds2_low16<F16>(p[y]), s[8 * kk + 2 * y + 1] - ds2_high16<F16>(p[y]));
+    return r;
+  };
   auto value_operand = [&](int buf, int half, int kk, int x) {
     const unsigned char* at = lv[buf] + v_lane + (half * 32 + kk * 16) * VROW + x * 64;
     const u32x2 w0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at));
@@ -451,10 +460,22 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
           const float offset1 = scores(n, st + 1 < ST ? buf : next, st + 1 < ST ? half + 1 : kg, key1);
           weights(s, off);
           const u32x4 p0 = packed(s, 0), p1 = packed(s, 1);
+          if constexpr (WIDE) {
+            const u32x4 r0 = rest(s, p0, 0), r1 = rest(s, p1, 1);
 #pragma unroll
-          for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
+            for (int x = 0; x < DB; ++x) {
+              const u32x4 v0 = value_operand(buf, half, 0, x), v1 = value_operand(buf, half, 1, x);
+              o[x] = mfma32<F16>(v0, p0, o[x]);
+              o[x] = mfma32<F16>(v1, p1, o[x]);
+              o[x] = mfma32<F16>(v0, r0, o[x]);
+              o[x] = mfma32<F16>(v1, r1, o[x]);
+            }
+          } else {
 #pragma unroll
-          for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 1, x), p1, o[x]);
+            for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 0, x), p0, o[x]);
+#pragma unroll
+            for (int x = 0; x < DB; ++x) o[x] = mfma32<F16>(value_operand(buf, half, 1, x), p1, o[x]);
+          }
           offset = exponents(n, key1, offset1);
           s = n;
         }
@@ -526,12 +547,15 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             const u32x4 p = packed(s, kk);
+            u32x4 r;
+            if constexpr (WIDE) r = rest(s, p, kk);
 #pragma unroll
             for (int x = 0; x < DB; ++x) {
               u32x4 v = value_operand(0, half, kk, x);
 #pragma unroll
               for (int y = 0; y < 4; ++y) v[y] &= edge ? ~not_finite<F16>(v[y]) : 0xffffffffu;
               o[x] = mfma32<F16>(v, p, o[x]);
+              if constexpr (WIDE) o[x] = mfma32<F16>(v, r, o[x]);
             }
           }
         }
@@ -591,25 +615,27 @@ __global__ __launch_bounds__(512, DP > 64 ? 2 : 4) void k_attn_masked(MaskedArgs
   }
 }
 
-template <bool F16, int DP, int KG>
+template <bool F16, int DP, int KG, bool WIDE>
 void launch_masked_mode(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
-  if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN, KG><<<dim3(blocks), 512, 0, st>>>(a);
-  else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP, KG><<<dim3(blocks), 512, 0, st>>>(a);
-  else if (mode == MASKED_LINEAR) k_attn_masked<F16, DP, MASKED_LINEAR, KG><<<dim3(blocks), 512, 0, st>>>(a);
-  else k_attn_masked<F16, DP, MASKED_GENERAL, KG><<<dim3(blocks), 512, 0, st>>>(a);
+  if (mode == MASKED_PLAIN) k_attn_masked<F16, DP, MASKED_PLAIN, KG, WIDE><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_CAP) k_attn_masked<F16, DP, MASKED_CAP, KG, WIDE><<<dim3(blocks), 512, 0, st>>>(a);
+  else if (mode == MASKED_LINEAR) k_attn_masked<F16, DP, MASKED_LINEAR, KG, WIDE><<<dim3(blocks), 512, 0, st>>>(a);
+  else k_attn_masked<F16, DP, MASKED_GENERAL, KG, WIDE><<<dim3(blocks), 512, 0, st>>>(a);
 }
-template <bool F16, int DP>
+template <bool F16, int DP, bool WIDE>
 void launch_masked_groups(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
-  if (a.key_groups == 2) launch_masked_mode<F16, DP, 2>(a, mode, blocks, st);
-  else launch_masked_mode<F16, DP, 1>(a, mode, blocks, st);
+  if constexpr (DP <= 128 && !WIDE) {
+    if (a.key_groups == 2) return launch_masked_mode<F16, DP, 2, WIDE>(a, mode, blocks, st);
+  }
+  launch_masked_mode<F16, DP, 1, WIDE>(a, mode, blocks, st);
 }
-template <bool F16>
+template <bool F16, bool WIDE = false>
 int launch_masked(const MaskedArgs& a, int mode, unsigned blocks, hipStream_t st) {
-  if (a.D <= 32) launch_masked_groups<F16, 32>(a, mode, blocks, st);
-  else if (a.D <= 64) launch_masked_groups<F16, 64>(a, mode, blocks, st);
-  else if (a.D <= 96) launch_masked_groups<F16, 96>(a, mode, blocks, st);
-  else if (a.D <= 128) launch_masked_groups<F16, 128>(a, mode, blocks, st);
-  else launch_masked_mode<F16, 256, 1>(a, mode, blocks, st);
+  if (a.D <= 32) launch_masked_groups<F16, 32, WIDE>(a, mode, blocks, st);
+  else if (a.D <= 64) launch_masked_groups<F16, 64, WIDE>(a, mode, blocks, st);
+  else if (a.D <= 96) launch_masked_groups<F16, 96, WIDE>(a, mode, blocks, st);
+  else if (a.D <= 128) launch_masked_groups<F16, 128, WIDE>(a, mode, blocks, st);
+  else launch_masked_groups<F16, 256, WIDE>(a, mode, blocks, st);
   DS2_CHECK_LAUNCH();
   return DS2_OK;
 }

@@ -41,10 +41,10 @@ Split split_of(const ds2_cache_attention_args& a) {
   if (a.prefix_len) {
     // A long prefix of many rows is a matrix product: the kernel of whole prompts takes it, whose key tiles in LDS serve 256 rows (16-bit
     // caches).  It costs a launch and more parts to join, so the product has to be large.
-    // 8 key heads, prompt kernel / this one: D = 64, 128 rows behind 32768 tokens 40 / 46 us, 256 behind 8192 30 / 26; D = 128, 128
-    // behind 32768 58 / 70, 64 behind 32768 52 / 45, 256 behind 8192 (and up to 512 tokens each) 57 / 50; D = 256, 32 behind 32768 78 / 67,
-    // 128 behind 8192 49 / 48, 256 behind 8192 66 / 86; one sequence of 64 tokens (256 rows a head, D = 128) behind 32768 77 / 105, of 512
-    // tokens 339 / 736.  (By sizes alone, whatever the queries' strides: the workspace goes by it.)
+    // 8 key heads, bf16, prompt kernel / this one: D = 64, 128 rows a head behind 32768 tokens 44 / 52 us, 256 54 / 61, 512 behind 8192
+    // 38 / 49; D = 128, 128 behind 32768 62 / 69, 256 86 / 114; D = 256, 256 behind 8192 70 / 80; smaller products are left here (of fp16, whose
+    // weights are one operand: 39 / 44, 49 / 60, 36 / 44; 57 / 67, 76 / 109; 65 / 74).  One sequence of 64 tokens (256 rows a head, D = 128) behind 32768
+    // 88 / 105, of 512 tokens 424 / 736.  (By sizes alone, whatever the queries' strides: the workspace goes by it.)
     const double product = (double)a.Hkv * all_rows * a.prefix_len * a.D;
     s.tiled = a.format == DS2_CACHE_PLAIN && product >= (a.D > 64 ? 3.0e9 : 1.8e9);
     if (s.tiled) {
@@ -179,7 +179,9 @@ extern "C" int ds2_op_cache_attention(const ds2_cache_attention_args* args, void
     m.key_groups = 1, m.row_tiles = s.pre_row_tiles, m.heads = x.Hkv, m.parts = s.pre_parts, m.tiles_a_part = s.pre_tiles;
     m.part_o = a.pre_o, m.part_ml = a.pre_ml;
     const unsigned tiles = (unsigned)(s.pre_row_tiles * x.Hkv * s.pre_parts);
-    DS2_TRY(f16 ? launch_masked_f16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st) : launch_masked_bf16(m, masked_mode(x.scale, x.cap, x.slopes), tiles, st));
+    // (bf16: weights of 16 bits like those over the sequences' own keys, so that a result's precision does not go by the prefix's size)
+    const int mode = masked_mode(x.scale, x.cap, x.slopes);
+    DS2_TRY(f16 ? launch_masked_f16(m, mode, tiles, st) : launch_masked_bf16_wide(m, mode, tiles, st));
   }
   DS2_TRY(x.format == DS2_CACHE_PLAIN ? launch_cache_attn_plain(a, f16, blocks, st)
           : x.format == DS2_CACHE_MXFP8 ? launch_cache_attn_mxfp8(a, f16, blocks, st)

@@ -16,7 +16,7 @@ import math
 import pytest
 import torch
 
-from test_hip_token_cache import DEV, cache_reference, masked_reference, ops, run_cache, run_masked  # noqa: F401
+from test_hip_token_cache import DEV, cache_reference, encode, masked_reference, ops, run_cache, run_masked  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +86,52 @@ def test_a_tail_far_below_one_key_of_a_cache(ops, case, gap):  # noqa: F811
     few = {**x, **{n: x[n][:2] for n in ("q", "k", "v")}}
     want, top, score = cache_reference(few, lens[:2], "plain", 1.0, 0.0, None, P)
     within(got[:2], want, top, score, torch.float16, 2.0 ** -11, 1, C + P, (C + P) * 60 * 2.0 ** -36)
+
+
+# ---- caches whose weights are two bf16 operands: their rounding is below the output's, whichever kernel takes the keys -----------------
+
+def peaked(g, *shape):
+    """Four elements of a query, scores of about +-5: a few keys have nearly all of the weight"""
+    q = torch.zeros(*shape)
+    q[..., :4] = 3 * torch.randn(*shape[:-1], 4, generator=g)
+    return q
+
+
+WIDE = [  # B, T, Hq, Hkv, D, C, P, cap, slopes, formats
+    (2, 1, 4, 2, 64, 500, 0, 0.0, False, "plain mxfp8 mxfp4"),
+    (2, 5, 8, 2, 128, 2000, 0, 0.0, False, "plain mxfp8 mxfp4"),
+    (3, 1, 8, 2, 256, 100, 333, 0.0, True, "plain mxfp8"),
+    (24, 1, 16, 2, 96, 40, 700, 30.0, False, "plain mxfp4"),
+    (32, 1, 16, 1, 32, 20, 9000, 0.0, False, "mxfp8"),
+    (128, 4, 32, 2, 32, 9, 3500, 0.0, False, "plain"),                 # the product over the prefix is large: the kernel of whole prompts
+    (128, 4, 32, 2, 64, 33, 1800, 0.0, False, "plain"),
+    (128, 4, 32, 2, 64, 33, 1800, 25.0, True, "plain"),
+    (128, 4, 32, 2, 64, 300, 1800, 0.0, True, "plain"),
+    (128, 4, 32, 2, 96, 33, 2000, 0.0, True, "plain"),
+    (128, 4, 32, 2, 128, 33, 1500, 25.0, False, "plain"),
+    (128, 4, 32, 2, 128, 33, 1500, 0.0, True, "plain"),
+    (128, 4, 32, 2, 256, 9, 800, 0.0, False, "plain"),
+    (128, 4, 32, 2, 256, 9, 800, 40.0, True, "plain"),
+    (1, 512, 32, 2, 64, 512, 1800, 0.0, False, "plain"),
+]
+
+
+@pytest.mark.parametrize("case,form", [(c, f) for c in WIDE for f in c[9].split()], ids=lambda c: c if isinstance(c, str) else "x".join(map(str, c[:9])))
+def test_weights_over_a_cache_of_bf16_have_16_bits(ops, case, form):  # noqa: F811
+    B, T, Hq, Hkv, D, C, P, cap, alibi, _ = case
+    g = torch.Generator().manual_seed(sum(case[:7]))
+    rows = lambda *lead: torch.randn(*lead, D, generator=g)  # noqa: E731
+    x = {"q": peaked(g, B, T, Hq, D).to(torch.bfloat16)}
+    for n, lead in (("k", (B, Hkv, C)), ("v", (B, Hkv, C)), ("pk", (Hkv, P)), ("pv", (Hkv, P))):
+        x[n], x[n + "s"] = (rows(*lead).to(torch.bfloat16), None) if form == "plain" else encode(rows(*lead), form)
+    lens = torch.tensor([max(T, C - 7 * b) for b in range(B)], dtype=torch.int32)
+    slopes = torch.exp2(-torch.arange(1, Hq + 1).float() * 8 / Hq) if alibi else None
+    got = run_cache(ops, x, lens, form, 1.0, cap, slopes, P)
+    few = {**x, **{n: None if x[n] is None else x[n][:6] for n in ("q", "k", "v", "ks", "vs")}}
+    want, top, _ = cache_reference(few, lens[:6], form, 1.0, cap, slopes, P)
+    # sizes of scores that have weight: their products, 30 of bias at most below the row's largest, 8 roundings of the cap
+    score = cache_reference(few, lens[:6], form, 1.0, 0.0, None, P)[2] + (30.0 if alibi else 0.0) + cap / 3
+    within(got[:6], want, top, score, torch.bfloat16, 2.0 ** -16, 4, C + P)
 
 
 # ---- positions far from the keys: what all keys of a row have in common is no part of a softmax -------------------------------------
