@@ -73,7 +73,7 @@ int check(const ds2_attention_masked_args& a) {
   DS2_REQUIRE(a.type == DS2_TYPE_BF16 || a.type == DS2_TYPE_F16, "attention_masked: bf16 or fp16 expected, got type %d", a.type);
   DS2_REQUIRE(std::isfinite(a.scale) && std::isfinite(a.cap) && a.cap >= 0.f, "attention_masked: scale and cap must be finite, cap not negative");
   DS2_REQUIRE(a.cap == 0.f || std::fabs(a.scale) <= 1e30f * a.cap, "attention_masked: the cap is too small for the scale");      // (scale / cap is a factor)
-  DS2_REQUIRE((!a.q_doc) == (!a.k_doc), "attention_masked: q_doc and k_doc go together");
+  DS2_REQUIRE((!a.q_doc) == (!a.k_doc) || !a.Lk, "attention_masked: q_doc and k_doc go together");      // (no keys: the documents of none are nowhere)
   DS2_REQUIRE(a.causal || !a.prefix, "attention_masked: a prefix goes with the causal mask");
   DS2_REQUIRE(a.Lk < (1 << 30) && (int64_t)(a.Hq / a.Hkv) * a.Lq < (1ll << 31) - 512, "attention_masked: sequence too long");
   DS2_REQUIRE((int64_t)a.B * a.Hkv < (1 << 24) && (int64_t)a.B * a.Lq * a.Hq < (1ll << 32), "attention_masked: too many rows for one call");

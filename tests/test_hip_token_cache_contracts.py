@@ -1,5 +1,5 @@
 """Calls of the token cache and its attention that the contracts allow, at their edges: one sequence with many new tokens behind a long prefix, queries
-in any order.  Plain forms: test_hip_token_cache.py."""
+in any order, no keys at all.  Plain forms: test_hip_token_cache.py."""
 import pytest
 import torch
 
@@ -30,3 +30,18 @@ def test_the_order_of_the_queries_changes_no_bit_behind_a_long_prefix(ops, B, T,
     q = x["q"].to(DEV)
     for view in (q.transpose(0, 1).contiguous().transpose(0, 1), q.transpose(1, 2).contiguous().transpose(1, 2), torch.cat((q, q), 1)[:, T:], torch.cat((q, q), -1)[..., :D]):
         assert torch.equal(view, q) and torch.equal(run_cache(ops, {**x, "q": view}, lens, "plain", D ** -0.5, 0.0, None, P), want)
+
+
+def test_no_keys_at_all(ops):  # noqa: F811
+    """Rows that see nothing are zero, with documents as without them."""
+    z = lambda *s: torch.ones(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
+    for B, Lq in ((1, 1), (2, 5), (3, 700)):
+        for causal in (True, False):
+            for doc in (None, (i32(B, Lq), i32(B, 0))):
+                out = ops.attention_masked(z(B, Lq, 4, 64), z(B, 0, 2, 64), z(B, 0, 2, 64), 1.0, causal, 0.0, None, i32(B), None, None, *(doc or (None, None)))
+                assert out.shape == (B, Lq, 4, 64) and not out.any()
+    with pytest.raises(RuntimeError, match="go together"):
+        ops.attention_masked(z(2, 5, 4, 64), z(2, 0, 2, 64), z(2, 0, 2, 64), 1.0, True, 0.0, None, None, None, None, i32(2, 5), None)
+    with pytest.raises(RuntimeError, match="k_doc must be"):
+        ops.attention_masked(z(2, 5, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), 1.0, True, 0.0, None, None, None, None, i32(2, 5), i32(2, 0))

@@ -1,7 +1,12 @@
 """What the C entries of the token cache and its attention promise about sizes, without a GPU."""
 import ctypes as C
 
-from test_token_cache_host import cache_args, lib, strided  # noqa: F401
+import pytest
+import torch
+
+from test_token_cache_host import FAKE, cache_args, lib, masked_args, masked_call, refused, strided  # noqa: F401
+
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are no GPU memory")
 
 
 def test_the_workspace_goes_by_the_sizes_alone(lib):  # noqa: F811
@@ -15,3 +20,12 @@ def test_the_workspace_goes_by_the_sizes_alone(lib):  # noqa: F811
                     need = {lib.ds2_op_cache_attention_work_bytes(C.byref(cache_args(q=q, **sizes)))
                             for q in (strided(T * row, row, D), strided(row, B * row, D), strided(0, row, D), strided(2 * T * row, row, D), strided(T * row, D, T * D), strided(0, 0, 0, p=None))}
                     assert len(need) == 1, (sizes, need)
+
+
+@no_gpu
+def test_documents_of_no_keys_need_no_memory(lib):  # noqa: F811
+    """The documents of an empty key axis are an empty tensor, which lies nowhere: what is refused below is the missing output, the next check."""
+    for q_doc in (FAKE, None):
+        refused(lib, masked_call(lib, Lk=0, q_doc=q_doc, k_doc=None, out=None), "output rows")
+        assert lib.ds2_op_attention_masked_work_bytes(C.byref(masked_args(Lk=0, q_doc=q_doc, k_doc=None))) == 0
+    refused(lib, masked_call(lib, Lk=1, q_doc=FAKE, k_doc=None, out=None), "go together")
