@@ -424,6 +424,14 @@ void no_overlap(const Tensor& t, const char* name) {
     need = ax[i].first * (ax[i].second - 1) + need;
   }
 }
+// These ops answer only: an input that requires a gradient would get none, silently.
+bool wants_gradient(const Tensor& t) { return t.requires_grad(); }
+bool wants_gradient(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+template <class... T>
+void no_backward(const char* op, const T&... inputs) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_gradient(inputs) || ...), "det_sam2::", op,
+              " has no backward pass: detach the inputs or call it under torch.no_grad()");
+}
 int64_t code_bytes(int32_t format, int64_t D) { return format == DS2_CACHE_MXFP4 ? D / 2 : D; }
 // lead axes and a last one
 void want_rows(const Tensor& t, at::IntArrayRef lead, int64_t last, const char* what, const char* name) {
@@ -441,6 +449,7 @@ void want_codes(const Tensor& c, const Tensor& s, at::IntArrayRef lead, int64_t 
 void cache_write(const Tensor& k, const c10::optional<Tensor>& v, const Tensor& pos, const c10::optional<Tensor>& count, Tensor k_codes,
                  Tensor k_scales, c10::optional<Tensor> v_codes, c10::optional<Tensor> v_scales, c10::string_view format) {
   const int32_t f = format_of(format, false), type = type_of(k, "k", true), n = v.has_value() ? 2 : 1;
+  no_backward("cache_write", k, v);
   TORCH_CHECK(v_codes.has_value() == v.has_value() && v_scales.has_value() == v.has_value(), "det_sam2::cache_write: v, v_codes and v_scales go together");
   TORCH_CHECK(k.dim() == 4 && k_codes.dim() == 4, "det_sam2::cache_write: k [B,T,H,D] and k_codes [B,H,C,D or D/2] expected");
   const auto dev = k.device();
@@ -491,6 +500,7 @@ Tensor cache_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
                        const c10::optional<Tensor>& prefix_v, const c10::optional<Tensor>& prefix_k_scales,
                        const c10::optional<Tensor>& prefix_v_scales, c10::string_view format, double scale, double cap,
                        const c10::optional<Tensor>& slopes) {
+  no_backward("cache_attention", q, k, v, prefix_k, prefix_v, slopes);
   ds2_cache_attention_args a{};
   a.format = format_of(format, true);
   a.type = type_of(q, "q", false);
@@ -544,6 +554,7 @@ Tensor cache_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
 Tensor attention_masked(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, double cap,
                         const c10::optional<Tensor>& slopes, const c10::optional<Tensor>& lens, const c10::optional<Tensor>& q_start,
                         const c10::optional<Tensor>& prefix, const c10::optional<Tensor>& q_doc, const c10::optional<Tensor>& k_doc) {
+  no_backward("attention_masked", q, k, v, slopes);
   ds2_attention_masked_args a{};
   a.type = type_of(q, "q", false);
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes(), "det_sam2::attention_masked: q [B,Lq,Hq,D], k / v [B,Lk,Hkv,D] expected");

@@ -1,5 +1,5 @@
 """Calls of the token cache and its attention that the contracts allow, at their edges: one sequence with many new tokens behind a long prefix, queries
-in any order, no keys at all.  Plain forms: test_hip_token_cache.py."""
+in any order, no keys at all, inputs that require gradients.  Plain forms: test_hip_token_cache.py."""
 import pytest
 import torch
 
@@ -45,3 +45,28 @@ def test_no_keys_at_all(ops):  # noqa: F811
         ops.attention_masked(z(2, 5, 4, 64), z(2, 0, 2, 64), z(2, 0, 2, 64), 1.0, True, 0.0, None, None, None, None, i32(2, 5), None)
     with pytest.raises(RuntimeError, match="k_doc must be"):
         ops.attention_masked(z(2, 5, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), 1.0, True, 0.0, None, None, None, None, i32(2, 5), i32(2, 0))
+
+
+def test_inputs_that_require_gradients_are_refused(ops):  # noqa: F811
+    """There is no backward pass: an answer without a gradient would be a gradient of zero to the caller."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8, device=DEV)  # noqa: E731
+    n = torch.ones(2, dtype=torch.int32, device=DEV)
+    slopes = torch.ones(4, device=DEV)
+    calls = {
+        "cache_write": (lambda k, v: ops.cache_write(k, v, n, None, u8(2, 2, 8, 64), u8(2, 2, 8, 2), u8(2, 2, 8, 64), u8(2, 2, 8, 2), "mxfp8"), [z(2, 3, 2, 64), z(2, 3, 2, 64)]),
+        "cache_attention": (lambda q, k, v, pk, pv, s: ops.cache_attention(q, k, v, None, None, n, pk, pv, None, None, "plain", 1.0, 0.0, s),
+                            [z(2, 1, 4, 64), z(2, 2, 8, 64), z(2, 2, 8, 64), z(2, 5, 64), z(2, 5, 64), slopes]),
+        "attention_masked": (lambda q, k, v, s: ops.attention_masked(q, k, v, 1.0, True, 0.0, s, None, None, None, None, None), [z(2, 5, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), slopes]),
+    }
+    for name, (call, inputs) in calls.items():
+        call(*inputs)
+        for i in range(len(inputs)):
+            some = [t.clone().requires_grad_(j == i) for j, t in enumerate(inputs)]
+            with pytest.raises(RuntimeError, match=f"{name} has no backward pass"):
+                call(*some)
+            with torch.no_grad():
+                call(*some)
+            with torch.inference_mode():
+                call(*some)
+            call(*(t.detach() for t in some))
