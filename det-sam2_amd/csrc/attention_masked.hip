@@ -75,7 +75,7 @@ int check(const ds2_attention_masked_args& a) {
   DS2_REQUIRE(a.cap == 0.f || std::fabs(a.scale) <= 1e30f * a.cap, "attention_masked: the cap is too small for the scale");      // (scale / cap is a factor)
   DS2_REQUIRE((!a.q_doc) == (!a.k_doc) || !a.Lk, "attention_masked: q_doc and k_doc go together");      // (no keys: the documents of none are nowhere)
   DS2_REQUIRE(a.causal || !a.prefix, "attention_masked: a prefix goes with the causal mask");
-  DS2_REQUIRE(a.Lk < (1 << 30) && (int64_t)(a.Hq / a.Hkv) * a.Lq < (1ll << 31) - 512, "attention_masked: sequence too long");
+  DS2_REQUIRE(a.Lk < (1 << 30) && a.Lq < (1 << 30) && (int64_t)(a.Hq / a.Hkv) * a.Lq < (1ll << 31) - 512, "attention_masked: sequence too long");
   DS2_REQUIRE((int64_t)a.B * a.Hkv < (1 << 24) && (int64_t)a.B * a.Lq * a.Hq < (1ll << 32), "attention_masked: too many rows for one call");
   return DS2_OK;
 }
@@ -106,7 +106,7 @@ extern "C" int ds2_op_attention_masked(const ds2_attention_masked_args* args, vo
     if (const int rc = aligned(x.v, "v")) return rc;
   }
   const Plan p = plan_of(x);
-  DS2_REQUIRE(p.blocks < (1ll << 31), "attention_masked: too many rows for one call");
+  DS2_REQUIRE(ds2_launch_holds(p.blocks, 512), "attention_masked: too many rows for one call");
   const int64_t need = p.doc_bytes + p.part_bytes;
   DS2_REQUIRE(!need || (work && (uintptr_t)work % 16 == 0 && work_bytes >= need), "attention_masked: workspace too small");
   MaskedArgs a{};
@@ -122,7 +122,7 @@ extern "C" int ds2_op_attention_masked(const ds2_attention_masked_args* args, vo
   hipStream_t st = (hipStream_t)stream;
   if (x.q_doc && p.tiles) {
     int2* docs = (int2*)work;
-    DS2_REQUIRE((int64_t)x.B * p.tiles < (1ll << 31), "attention_masked: too many keys for one call");
+    DS2_REQUIRE(ds2_launch_holds((int64_t)x.B * p.tiles, 64), "attention_masked: too many keys for one call");
     if (masked_tile(x.D) == 64) k_tile_docs<64><<<dim3((unsigned)(x.B * p.tiles)), 64, 0, st>>>(x.k_doc, x.Lk, p.tiles, docs);
     else k_tile_docs<32><<<dim3((unsigned)(x.B * p.tiles)), 64, 0, st>>>(x.k_doc, x.Lk, p.tiles, docs);
     DS2_CHECK_LAUNCH();

@@ -98,7 +98,7 @@ int check(const ds2_cache_attention_args& a) {
   DS2_REQUIRE((int64_t)a.capacity + a.prefix_len < (1ll << 31) - 4096 && a.T < (1 << 20), "cache_attention: too many tokens");
   DS2_REQUIRE((int64_t)a.B * a.T * a.Hq < (1ll << 31) / 256, "cache_attention: too many rows (B T Hq) for one call");
   const Split s = split_of(a);
-  DS2_REQUIRE(s.blocks < (1ll << 31) && s.streams * (cdiv64(a.capacity, CACHE_UNIT) + 1) < (1ll << 31) - 4096, "cache_attention: too many keys for one call");
+  DS2_REQUIRE(ds2_launch_holds(s.blocks, 256) && ds2_launch_holds((int64_t)s.pre_row_tiles * a.Hkv * s.pre_parts, 512) && s.streams * (cdiv64(a.capacity, CACHE_UNIT) + 1) < (1ll << 31) - 4096, "cache_attention: too many keys for one call");
   return DS2_OK;
 }
 

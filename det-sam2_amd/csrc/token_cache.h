@@ -10,6 +10,8 @@
 
 #define DS2_CACHE_GROUP 32
 #define DS2_CAP_WIDE 256.f
+// a launch holds fewer than 2^32 threads
+inline bool ds2_launch_holds(int64_t blocks, int threads) { return blocks <= 0xffffffffll / threads; }
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));

@@ -182,8 +182,9 @@ extern "C" int ds2_op_cache_write(int32_t n, const ds2_strided* x, const ds2_str
     a.x[i] = x[i], a.codes[i] = codes[i], a.scales[i] = scales[i];
   }
   a.pos = pos, a.count = count, a.T = T, a.H = H, a.D = D, a.capacity = capacity;
+  DS2_REQUIRE((int64_t)T * (D / 8) < (1ll << 31) - 1024 && (int64_t)B * H < (1ll << 24), "cache_write: too many rows for one call");
   const int64_t per = cdiv64((int64_t)T * (D / 8), 1024), blocks = per * n * B * H;
-  DS2_REQUIRE((int64_t)T * (D / 8) < (1ll << 31) - 1024 && blocks < (1ll << 31) && (int64_t)n * B * H < (1ll << 31), "cache_write: too many rows for one call");
+  DS2_REQUIRE(ds2_launch_holds(blocks, 256), "cache_write: too many rows for one call");
   a.BH = B * H, a.blocks_per_head = (int)per;
   hipStream_t st = (hipStream_t)stream;
 #define GO(TY, F) k_cache_write<TY, F><<<dim3((unsigned)blocks), 256, 0, st>>>(a)
@@ -206,8 +207,9 @@ extern "C" int ds2_op_cache_read(const ds2_strided* codes, const ds2_strided* sc
   DS2_REQUIRE(codes->p && scales->p && out->p, "cache_read: null pointer");
   DS2_REQUIRE(aligned(*codes, 1, 16, 3) && aligned(*out, type == DS2_TYPE_F32 ? 4 : 2, 16, 3), "cache_read: rows must be 16-byte aligned");
   ReadArgs a{*codes, *scales, *out, lens, C, H, D, 0, 256 / (D / 8), 256 % (D / 8)};
+  DS2_REQUIRE((int64_t)C * (D / 8) < (1ll << 31) - 1024 && (int64_t)B * H < (1ll << 24), "cache_read: too many rows for one call");
   const int64_t per = cdiv64((int64_t)C * (D / 8), 1024), blocks = per * B * H;
-  DS2_REQUIRE((int64_t)C * (D / 8) < (1ll << 31) - 1024 && blocks < (1ll << 31) && (int64_t)B * H < (1ll << 31), "cache_read: too many rows for one call");
+  DS2_REQUIRE(ds2_launch_holds(blocks, 256), "cache_read: too many rows for one call");
   a.blocks_per_head = (int)per;
   hipStream_t st = (hipStream_t)stream;
 #define GO(TY, F) k_cache_read<TY, F><<<dim3((unsigned)blocks), 256, 0, st>>>(a)

@@ -1,10 +1,11 @@
-"""What the C entries of the token cache and its attention promise about sizes, without a GPU."""
+"""What the C entries of the token cache and its attention promise about sizes, without a GPU: workspaces that go by the sizes alone, calls
+that are too large for one launch or one index."""
 import ctypes as C
 
 import pytest
 import torch
 
-from test_token_cache_host import FAKE, cache_args, lib, masked_args, masked_call, refused, strided  # noqa: F401
+from test_token_cache_host import FAKE, cache_args, cache_call, lib, masked_args, masked_call, read, refused, strided, write  # noqa: F401
 
 no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are no GPU memory")
 
@@ -29,3 +30,31 @@ def test_documents_of_no_keys_need_no_memory(lib):  # noqa: F811
         refused(lib, masked_call(lib, Lk=0, q_doc=q_doc, k_doc=None, out=None), "output rows")
         assert lib.ds2_op_attention_masked_work_bytes(C.byref(masked_args(Lk=0, q_doc=q_doc, k_doc=None))) == 0
     refused(lib, masked_call(lib, Lk=1, q_doc=FAKE, k_doc=None, out=None), "go together")
+
+
+@no_gpu
+@pytest.mark.parametrize("change", [dict(B=1 << 22, H=4, T=1, D=32), dict(B=1 << 12, H=1, T=1 << 15, D=4096), dict(n=2, B=1 << 23, H=1, T=1, D=32)])
+def test_a_write_of_more_rows_than_a_launch_holds_is_refused(lib, change):  # noqa: F811
+    refused(lib, write(lib, **change), "too many rows")
+
+
+@no_gpu
+@pytest.mark.parametrize("change", [dict(B=1 << 22, H=4, C_=1, D=32), dict(B=1 << 12, H=1, C_=1 << 15, D=4096)])
+def test_a_read_of_more_rows_than_a_launch_holds_is_refused(lib, change):  # noqa: F811
+    refused(lib, read(lib, **change), "too many rows")
+
+
+@no_gpu
+@pytest.mark.parametrize("change,match", [
+    (dict(B=1 << 20, Hq=8, Hkv=8, Lq=1, Lk=1), "too many rows"),                            # 2^23 workgroups of 512 threads
+    (dict(B=1, Hq=1, Hkv=1, Lq=1 << 30, D=8), "too long"),                                  # a position that no 32-bit number holds
+    (dict(B=1, Hq=1, Hkv=1, Lq=(1 << 30) + (1 << 29), D=8), "too long"),
+    (dict(B=1 << 22, Hq=1, Hkv=1, Lq=1, Lk=1024, D=8, q_doc=FAKE, k_doc=FAKE), "too many keys"),   # 2^26 tiles of documents, a workgroup of 64 threads each
+])
+def test_prompts_beyond_a_launch_are_refused(lib, change, match):  # noqa: F811
+    refused(lib, masked_call(lib, **change), match)
+
+
+@no_gpu
+def test_a_cache_beyond_a_launch_is_refused(lib):  # noqa: F811
+    refused(lib, cache_call(lib, B=1 << 20, Hq=4, Hkv=4, T=1, capacity=1, prefix_len=1 << 20, format=1), "too many")
