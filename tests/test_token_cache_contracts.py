@@ -1,10 +1,15 @@
 """What the C entries of the token cache and its attention promise about sizes, without a GPU: workspaces that go by the sizes alone, calls
-that are too large for one launch or one index."""
+that are too large for one launch or one index, and the registers of the built kernels."""
 import ctypes as C
+import os
+import re
+import struct
+import subprocess
 
 import pytest
 import torch
 
+from det_sam2_amd import _capi
 from test_token_cache_host import FAKE, cache_args, cache_call, lib, masked_args, masked_call, read, refused, strided, write  # noqa: F401
 
 no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are no GPU memory")
@@ -58,3 +63,36 @@ def test_prompts_beyond_a_launch_are_refused(lib, change, match):  # noqa: F811
 @no_gpu
 def test_a_cache_beyond_a_launch_is_refused(lib):  # noqa: F811
     refused(lib, cache_call(lib, B=1 << 20, Hq=4, Hkv=4, T=1, capacity=1, prefix_len=1 << 20, format=1), "too many")
+
+
+# ---- the built kernels ----------------------------------------------------------------------------------------------------------
+
+READELF = "/opt/rocm/llvm/bin/llvm-readelf"
+
+
+def kernels(path):
+    """name and place of each kernel -> its entry in the metadata of the library's gfx950 code objects"""
+    raw, magic, at, out = open(path, "rb").read(), b"__CLANG_OFFLOAD_BUNDLE__", 0, {}
+    while (at := raw.find(magic, at)) >= 0:
+        (count,), p = struct.unpack_from("<Q", raw, at + 24), at + 32
+        for _ in range(count):
+            offset, size, n = struct.unpack_from("<QQQ", raw, p)
+            name, p = raw[p + 24:p + 24 + n], p + 24 + n
+            if b"gfx950" in name and size:
+                text = subprocess.run([READELF, "--notes", "-"], input=raw[at + offset:at + offset + size], stdout=subprocess.PIPE, check=True).stdout.decode()
+                for entry in re.split(r"\n  - (?=\.agpr_count)", text)[1:]:
+                    out[re.search(r"\.name:\s+(\S+)", entry).group(1), at] = entry
+        at += len(magic)
+    return out
+
+
+@pytest.mark.skipif(not os.path.exists(READELF), reason="no llvm-readelf")
+def test_the_attention_kernels_hold_no_accumulator_registers(lib):  # noqa: F811
+    """hipcc has left out wait states in front of copies from accumulator registers, and has put copies into them in front of the restored lane
+    mask of a divergent branch.  Launch bounds keep these kernels out of those registers; a rebuild that does not is seen here."""
+    found = {n: e for n, e in kernels(_capi.LIB_PATH).items() if any(k in n[0] for k in ("k_attn_masked", "k_cache_attn", "k_attn_join"))}
+    assert len([n for n in found if "k_attn_masked" in n[0]]) >= 92 and len([n for n in found if "k_cache_attn" in n[0]]) >= 30
+    number = lambda e, key: int(re.search(rf"\.{key}:\s+(\d+)", e).group(1))  # noqa: E731
+    for name, entry in found.items():
+        assert number(entry, "agpr_count") == 0, name
+        assert number(entry, "vgpr_count") <= 256, name
