@@ -36,7 +36,10 @@ Plan plan_of(const ds2_attention_masked_args& a) {
   // long as the longest workgroup or the work of a CU; parts cost a join, 7 us and what they write and read at 4 TB/s.  Measured, rows
   // whole / keys split over waves: 32 over 8 heads, D = 128, causal 1024 tokens 39 / 30 us, 2048 tokens 75 / 61, four times 2048
   // of 16 over 8 heads 98 / 123; D = 96, twice 2500 tokens of 8 over 4 heads 71 / 51.  Parts: 4 over 1 heads, D = 64, 4096 tokens over
-  // 28736 in eight parts 175 us, two 332; the 1024 tokens above in one part 39, four 60.
+  // 28736 in eight parts 175 us, two 332; the 1024 tokens above in one part 39, four 60.  More than 64 parts, up to as many as CUs, where each
+  // keeps 1024 keys (64 / as many as CUs): 16 tokens of 4 over 1 heads, D = 64, over 2^20 keys 258 / 83 us; 64 tokens, D = 128, over 2^18
+  // 94 / 65; 16 of 8 over 2 heads, D = 128, over 2^18 93 / 63.  Shorter parts gain nothing (64 tokens of 8 over 1 heads, D = 128, over 2^16
+  // 38.5 / 37; 77 of 4 over 2, D = 64, over 40000 23.7 / 23.4).
   const double part_us = (double)a.B * a.Lq * a.Hq * a.D * 8 / 4e6, step_us = a.D > 128 ? 1.8 : a.D > 96 ? 1.15 : a.D > 64 ? 1.0 : 0.8;
   const double seen = a.causal && a.Lk ? 1 - 0.5 * std::min(1.0, (double)a.Lq / a.Lk) : 1;      // of all pairs
   // Tiles of a row.  How long documents are is known to the device only, which splits what a tile of rows can see; half of all keys is
@@ -47,7 +50,7 @@ Plan plan_of(const ds2_attention_masked_args& a) {
   p.parts = p.key_groups = 1;
   for (int kg = 1; kg <= (a.D <= 128 ? 2 : 1); ++kg) {
     const int64_t whole = cdiv64(rows, masked_rows(a.D, kg)) * p.heads;
-    const int most = whole < 256 ? std::max(1, std::min(reach / 2, 64)) : 1;
+    const int most = whole < 256 ? std::max(1, std::max(std::min(reach / 2, 64), std::min((int)cdiv64(256, whole), reach * masked_tile(a.D) / 1024))) : 1;
     for (int n = 1; n <= most; n += 1 + n / 8) {
       const double longest = (double)cdiv(reach, n) * (masked_tile(a.D) / 32) / kg;
       const double on_cu = seen < 1 ? whole * n / 256.0 : (double)cdiv64(whole * n, 256);

@@ -3,7 +3,7 @@ in any order, no keys at all, inputs that require gradients.  Plain forms: test_
 import pytest
 import torch
 
-from test_hip_token_cache import DEV, cache_case, cache_reference, near, ops, run_cache  # noqa: F401
+from test_hip_token_cache import DEV, cache_case, cache_reference, masked_reference, near, ops, run_cache, run_masked, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -30,6 +30,17 @@ def test_the_order_of_the_queries_changes_no_bit_behind_a_long_prefix(ops, B, T,
     q = x["q"].to(DEV)
     for view in (q.transpose(0, 1).contiguous().transpose(0, 1), q.transpose(1, 2).contiguous().transpose(1, 2), torch.cat((q, q), 1)[:, T:], torch.cat((q, q), -1)[..., :D]):
         assert torch.equal(view, q) and torch.equal(run_cache(ops, {**x, "q": view}, lens, "plain", D ** -0.5, 0.0, None, P), want)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv,D,causal,alibi", [(5, 90000, 4, 1, 64, False, False), (3, 133000, 2, 1, 128, True, True), (2, 100011, 2, 2, 256, False, False)])
+def test_a_row_of_more_than_64_parts(ops, Lq, Lk, Hq, Hkv, D, causal, alibi, kind):  # noqa: F811
+    g = torch.Generator().manual_seed(D)
+    q, k, v = torch.randn(1, Lq, Hq, D, generator=g).to(kind), values(g, 1, Lk, Hkv, D, kind=kind), values(g, 1, Lk, Hkv, D, kind=kind)
+    slopes = torch.exp2(-6 - torch.arange(1, Hq + 1).float() * 8 / Hq) if alibi else None
+    args = (D ** -0.5, causal, 0.0, slopes, torch.tensor([Lk - 1000], dtype=torch.int32), torch.tensor([Lk - Lq], dtype=torch.int32), None, None)
+    want, top, score = masked_reference(q, k, v, *args)
+    near(run_masked(ops, q, k, v, *args), want, top, score, kind)
 
 
 def test_no_keys_at_all(ops):  # noqa: F811

@@ -65,6 +65,14 @@ def test_a_cache_beyond_a_launch_is_refused(lib):  # noqa: F811
     refused(lib, cache_call(lib, B=1 << 20, Hq=4, Hkv=4, T=1, capacity=1, prefix_len=1 << 20, format=1), "too many")
 
 
+@pytest.mark.parametrize("Lq,Lk,Hq,Hkv,D,least", [(16, 1 << 20, 4, 1, 64, 200), (64, 1 << 18, 4, 1, 128, 200), (16, 1 << 18, 8, 2, 128, 100), (16, 1 << 17, 4, 1, 256, 100), (16, 1 << 18, 4, 1, 256, 200)])
+def test_few_rows_over_many_keys_are_split_over_the_chip(lib, Lq, Lk, Hq, Hkv, D, least):  # noqa: F811
+    """256 compute units: as many parts as there are units for each tile of rows, as far as the model of the split goes (the workspace tells)."""
+    n = lib.ds2_op_attention_masked_work_bytes(C.byref(masked_args(B=1, Lq=Lq, Lk=Lk, Hq=Hq, Hkv=Hkv, D=D, causal=0)))
+    parts = n / (Lq * Hq * (D + 2) * 4)
+    assert parts == int(parts) and least <= parts <= 256 // Hkv
+
+
 # ---- the built kernels ----------------------------------------------------------------------------------------------------------
 
 READELF = "/opt/rocm/llvm/bin/llvm-readelf"
