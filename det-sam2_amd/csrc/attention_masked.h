@@ -28,11 +28,12 @@
 //    take up to a fifth more time (8 key heads, 2048 rows a head behind 8192 tokens: D = 64 69 -> 84 us, D = 128 105 -> 127).  A prefix that
 //    sequences share has them, as their own tokens do; whole prompts have one.
 //
-// Measured (16-bit operands in, TFLOP/s over the visible pairs): D = 128, 32 over 8 heads, 8192 tokens: full 967, causal 945, capped
-// 830, distance bias 895; a plain library product of 16-bit matrices makes 1096 on the same card.  D = 64, 16 heads, 8190 tokens: 730,
-// causal 637; D = 256, 8 over 2 heads, 4096 tokens: 595.  At D = 128 the matrix pipes are busy 43 % of the cycles, the vector pipe
-// 39 %, LDS 27 %; other orders of a step, priorities, and halves of the workgroup in opposite phases all took the same time or more.
-// At D = 64 the exponentials (a quarter of the vector rate) carry more weight: vector pipe 68 %, matrix pipes 41 %.
+// Measured (fp16 / bf16 operands, normal values, TFLOP/s over the visible pairs): D = 128, 32 over 8 heads, 8192 tokens: full 962 / 1014, causal 928 /
+// 974, capped 817 / 851, distance bias 871 / 900; a plain library product of such matrices makes 1035 / 1096 on the same card.  D = 64, 16 heads, 8190
+// tokens: 865 / 902, causal 671 / 690, bias 702 / 739; D = 256, 8 over 2 heads, 4096 tokens: 592 / 619 (both waves of a row compute its scores: three
+// units of matrix work in place of two).  At D = 128 the matrix pipes are busy 44 % of the cycles, the vector pipe 39 %, LDS 27 %; other orders
+// of a step, priorities, and halves of the workgroup in opposite phases all took the same time or more.  At D = 64 the exponentials (a quarter of the
+// vector rate) carry more weight: vector pipe 67 %, matrix pipes 41 %.
 #pragma once
 #include "token_cache.h"
 
@@ -49,7 +50,8 @@ constexpr int masked_rows(int D, int key_groups) { return 256 / masked_value_spl
 constexpr int masked_tile(int D) { return D > 128 ? 32 : 64; }   // keys of a tile
 constexpr float LOG2E = 1.44269504088896340736f;
 // How scores become exponents.  LINEAR: distance bias without a cap, by what the products start from; GENERAL: cap and bias, or a scale
-// or cap that the others do not take.  (D = 64, 16 heads, 8190 tokens with a bias: GENERAL 659 TFLOP/s, LINEAR 727, PLAIN without it 726.)
+// or cap that the others do not take.  (D = 64, 16 heads, 8190 tokens, fp16 / bf16 TFLOP/s: with a bias GENERAL 634 / 666, LINEAR 679 /
+// 736; without GENERAL 725 / 754, PLAIN 833 / 881; capped GENERAL with a bias 490 / 503, CAP without 619 / 633.)
 enum { MASKED_PLAIN = 0, MASKED_CAP = 1, MASKED_LINEAR = 2, MASKED_GENERAL = 3 };
 
 }  // namespace

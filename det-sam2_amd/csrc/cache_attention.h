@@ -36,11 +36,13 @@
 //    workgroups are in one launch with the sequences' own; a large product over a 16-bit prefix goes to the kernel of whole prompts
 //    instead.
 //
-// Measured: 32 sequences of 8192 tokens, 8 key heads of 128: 16 bits 191 us, 5.6 TB/s of cache; 8 bits 108 us, 5.1 TB/s; 4 bits 66 us, 4.3
-// TB/s (64 sequences, heads of 64: 186, 107, 74 us).  A large copy makes 4.9 TB/s, a sum over a large tensor 6.0.  Ragged, 65 to 8192
-// tokens, 8 bits: 63.5 us, 5.0 TB/s with the join.  Four bits are bound by the vector pipe (61 % busy at D = 64: 215 instructions a block
-// of 32 keys, mostly conversions and the turning of values), the others by memory.  One sequence of 1501 tokens, 8 key heads: 8 us and
-// 3.5 for the join, all of it latency.
+// Measured: 32 sequences of 8192 tokens, 8 key heads of 128: 16 bits 194 us, 5.5 TB/s of cache; 8 bits 109 us, 5.1 TB/s; 4 bits 67 us, 4.2
+// TB/s (64 sequences, heads of 64: 188, 108, 77 us).  A large copy makes 4.9 TB/s, a sum over a large tensor 6.0.  Ragged, 65 to 8192
+// tokens, 8 bits: 65 us, 4.3 TB/s with the join.  Four bits are bound by the vector pipe (60 % busy at D = 64: 215 instructions a block
+// of 32 keys, mostly conversions and the turning of values), the others by memory.  One sequence of 2048 tokens, 8 key heads: 8 us and
+// 3.5 for the join, all of it latency.  64 sequences of 33 to 512 tokens behind 8192 (16 bits, 8 heads of 128, 4 query heads each): 46 us and
+// 4.5 for the join; no pipe is full (vector 30 % of cycles, matrix 11 %, vector memory 33 %): the 16 row groups of a head's 256 rows take the
+// prefix's 33.5 MB through L1 16 times, and on average half of the waves that fit are resident.
 #pragma once
 #include <algorithm>
 

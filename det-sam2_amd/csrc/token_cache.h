@@ -26,7 +26,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 // so.  bf16 has the exponents of fp32 and needs none.  fp16 ends at 2^16 and loses bits below 2^-14: with weights of 2^11 to 2^15 for
 // the largest, 11 bits remain down to 2^-25 of it, and below that no weight is off by more than 2^-36 of it.  (References at the largest score and a
 // limit of 2^8: 11 bits down to 2^-14, nothing at all below 2^-25.  Where the largest weight falls on a value of zero and the others are e^-17.5 of
-// it, the row was off by 10 to 40 half steps of the output.)  Raising after 2^4 and not 2^8 costs 3 % where
+// it, rows were off by 1 to 5 %.)  Raising after 2^4 and not 2^8 costs 3 % where
 // a bias lets the scores climb from key to key (4096 rows over 28736 keys, D = 64: 182 -> 187 us); elsewhere it is rare after a row's first keys.
 template <bool F16>
 constexpr float DS2_SHIFT = F16 ? 11.f : 0.f;

@@ -346,7 +346,11 @@ int ds2_op_cache_read(const ds2_strided* codes, const ds2_strided* scales, const
  * among them (below 0 counts as 0, beyond the capacity as the capacity); new token t sees the prefix and its own tokens up to lens[b] - T + t; where that is negative it sees nothing.
  * prefix_* [Hkv,prefix_len,D] (axes -,h,token; s0 is not used), or prefix_len = 0.  slopes fp32 [Hq] or NULL.  Rows that see nothing are
  * zero.  out [B,T,Hq,D] contiguous, q's type.  D = 32, 64, 96, 128 or 256; all rows 16-byte aligned (scales: any).
- * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), 16-byte aligned, which goes by the sizes alone;
+ * Scores, weights' sums and results are fp32 until the one rounding to q's type; for the product with the values a weight has 16 bits, over a cache
+ * of fp16 11 (down to 2^-25 of the row's largest, none is off by more than 2^-36 of it).  The sums hold weights of up to 2^15 times values: bf16
+ * values beyond 2^100 may overflow them.
+ * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), 16-byte aligned, which goes by sizes, type and format
+ * alone (B to format of the struct), not by strides;
  * two calls that may run at once need two of them.  The stream is the caller's, the device the current one; nothing synchronises. */
 typedef struct ds2_cache_attention_args {
   int32_t B, T, Hq, Hkv, D, capacity, prefix_len, type, format;
@@ -365,8 +369,9 @@ int ds2_op_cache_attention(const ds2_cache_attention_args* args, void* work, int
  *   j < lens[b]                                   (lens int32 [B] or NULL), and
  *   j <= q_start[b] + i or j < prefix[b]          where causal (prefix int32 [B] or NULL), and
  *   q_doc[b,i] == k_doc[b,j] and k_doc[b,j] >= 0  where documents are given (int32 [B,Lq] / [B,Lk] contiguous, in any order).
- * Rows that see nothing are zero.  D a multiple of 8 up to 256; all rows 16-byte aligned.
- * work: as above, of ds2_op_attention_masked_work_bytes(args) bytes. */
+ * Rows that see nothing are zero.  D a multiple of 8 up to 256; Lq and Lk below 2^30; all rows 16-byte aligned.  Where Lk is 0 the documents of the
+ * keys may be NULL.  Precision as above, weights with the operands' bits (bf16 8, fp16 11) for the product with the values.
+ * work: as above, of ds2_op_attention_masked_work_bytes(args) bytes, which go by the sizes, by `causal` and by whether documents are given. */
 typedef struct ds2_attention_masked_args {
   int32_t B, Lq, Lk, Hq, Hkv, D, type, causal;
   float scale, cap;
