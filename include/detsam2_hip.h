@@ -348,7 +348,7 @@ int ds2_op_cache_read(const ds2_strided* codes, const ds2_strided* scales, const
  * zero.  out [B,T,Hq,D] contiguous, q's type.  D = 32, 64, 96, 128 or 256; all rows 16-byte aligned (scales: any).
  * Scores, weights' sums and results are fp32 until the one rounding to q's type; for the product with the values a weight has 16 bits, over a cache
  * of fp16 11 (down to 2^-25 of the row's largest, none is off by more than 2^-36 of it).  The sums hold weights of up to 2^15 times values: bf16
- * values beyond 2^100 may overflow them.
+ * values beyond 2^100 may overflow them, and scores beyond 2^27 in magnitude, with their bias, are out of range.
  * work: device scratch of ds2_op_cache_attention_work_bytes(args) bytes (0: none needed), 16-byte aligned, which goes by sizes, type and format
  * alone (B to format of the struct), not by strides;
  * two calls that may run at once need two of them.  The stream is the caller's, the device the current one; nothing synchronises. */

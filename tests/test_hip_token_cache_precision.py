@@ -153,3 +153,36 @@ def test_queries_far_from_the_keys(ops, D, Lq, Lk, start, causal, cap, kind):  #
     got = ops.attention_masked(q.to(DEV), k.to(DEV), v.to(DEV), D ** -0.5, causal, cap, slopes.to(DEV), lens.to(DEV),
                                torch.tensor(start, dtype=torch.int32, device=DEV), None, None, None)
     within(got, want, top, score, kind, torch.finfo(kind).eps / 2, D, Lk, Lk * float(v.abs().max()) * 2.0 ** -36)
+
+
+# ---- scores so large that fp32 holds no fraction of them --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 11, 2.0 ** 12.5])
+@pytest.mark.parametrize("D,mode", [(64, "plain"), (128, "plain"), (256, "plain"), (64, "bias"), (128, "bias"), (64, "negative")])
+def test_scores_without_a_fraction(ops, D, mode, size, kind):  # noqa: F811
+    """Scores of up to 2^26: neighbouring fp32 numbers are up to 8 apart, and so are products and references.  The largest score is alone by far
+    more than that, and its value is the answer: its weight is a power of 2 with any fraction, rounded for the product, not in the sum."""
+    g = torch.Generator().manual_seed(D)
+    Lq, Lk = 70, 500
+    q, k = torch.zeros(2, Lq, 2, D), torch.zeros(2, Lk, 1, D)
+    q[..., 0] = size * (1 + torch.arange(Lq).view(1, Lq, 1) / 128)                   # (8 bits)
+    k[..., 0] = size * (1 + torch.stack([torch.randperm(Lk, generator=g) for _ in range(2)]).view(2, Lk, 1) % 128 / 128)
+    best = k[:, :, 0, 0].argmax(1)
+    for b in range(2):                                                               # one largest key, the others at most half of it
+        k[b, :, 0, 0] /= 2
+        k[b, best[b], 0, 0] *= 2
+    q, k, v = q.to(kind), k.to(kind), torch.randn(2, Lk, 1, D, generator=g).to(kind)
+    scale = -1.0 if mode == "negative" else 1.0
+    k = -k if mode == "negative" else k
+    want = v[torch.arange(2), best, 0].view(2, 1, 1, D).expand(2, Lq, 2, D)
+    slopes = torch.tensor([0.25, 2.0 ** -6], device=DEV) if mode == "bias" else None
+    d = [t.to(DEV) for t in (q, k, v)]
+    got = ops.attention_masked(*d, scale, False, 0.0, slopes, None, None, None, None, None)
+    u, none = torch.finfo(kind).eps / 2, torch.zeros(want.shape[:-1], dtype=torch.float64)
+    within(got, want.double(), want.double().abs(), none, kind, u, 1, Lk)
+    if mode != "negative" and D != 128:
+        lens = torch.full((2,), Lk, dtype=torch.int32, device=DEV)
+        head_major = [t.transpose(1, 2).contiguous() for t in d[1:]]
+        got = ops.cache_attention(d[0][:, -1:], *head_major, None, None, lens, None, None, None, None, "plain", scale, 0.0, slopes)
+        within(got, want[:, -1:].double(), want[:, -1:].double().abs(), none[:, -1:], kind, u, 1, Lk)
